@@ -43,6 +43,16 @@ SIGNATURES = {
                                                              _c_void_p]),
     "afa_decode_workspace_bytes": (_c_size, [_c_int] * 4),
     "afa_decode_noalloc": (_c_int, [_c_void_p] * 5 + [_c_int] * 5 + [_c_float, _c_void_p, _c_int, _c_void_p]),
+    "afa_paged_plan": (_c_int, [_c_void_p] * 16 + [_c_int] * 6 + [_c_void_p]),
+    "afa_ago_rotate_axes": (_c_int, [_c_void_p] * 3 + [_c_int] + [_c_void_p] * 3 + [_c_int] + [_c_void_p] * 2 +
+                            [_c_int] * 2 + [_c_void_p] * 2 + [_c_int] + [_c_void_p] + [_c_int] * 7 + [_c_void_p]),
+    "afa_paged_append": (_c_int, [_c_void_p] * 12 + [_c_int] + [_c_void_p] * 2 + [_c_int] * 2 + [_c_void_p] * 2 +
+                         [_c_int] + [_c_void_p] + [_c_int] * 7 + [_c_void_p]),
+    "afa_paged_commit": (_c_int, [_c_void_p] * 5 + [_c_ll] + [_c_void_p] * 3 + [_c_ll, _c_void_p] + [_c_int] * 9 +
+                         [_c_void_p]),
+    "afa_paged": (_c_int, [_c_void_p] * 9 + [_c_ll] + [_c_void_p] * 3 + [_c_ll] + [_c_int] * 10 +
+                  [_c_float, _c_void_p, _c_size, _c_void_p]),
+    "afa_paged_workspace_bytes": (_c_size, [_c_int] * 5),
     "algebraic_softmax_fwd": (_c_int, [_c_void_p, _c_void_p, _c_ll, _c_int, _c_int, _c_double, _c_double,
                                        _c_void_p]),
     "algebraic_softmax_bwd": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_ll, _c_int, _c_int, _c_double, _c_double,

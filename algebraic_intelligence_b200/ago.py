@@ -10,8 +10,13 @@ reference's signatures (src/attention.py:93-240):
                                    prologue of the attention layer
                                    (src/model.py:262-264)
 
-Both run as CUDA kernels (``afa_ago_table`` / ``afa_ago_rotate``): the tables by
-a per-pair recurrence over positions, the rotation as one pass over q and k.
+* ``apply_ago_rotations_axes``   -- the rotation with several position axes
+                                   (time, height, width), differentiable; no
+                                   reference counterpart
+
+All run as CUDA kernels (``afa_ago_table`` / ``afa_ago_rotate`` /
+``afa_ago_rotate_axes``): the tables by a per-pair recurrence over positions,
+the rotations as one pass over q and k.
 """
 from __future__ import annotations
 
@@ -24,7 +29,7 @@ import torch
 from . import _lib
 from ._tensors import Staged, host_checks_float
 
-__all__ = ["CayleyRotary", "build_cayley_rotary_matrix", "apply_ago_rotations"]
+__all__ = ["CayleyRotary", "build_cayley_rotary_matrix", "apply_ago_rotations", "apply_ago_rotations_axes"]
 
 
 class CayleyRotary(NamedTuple):
@@ -157,3 +162,148 @@ def apply_ago_rotations(q, k, rotary_params=None, seq_axis: Optional[int] = None
                                         inner, _lib.dtype_code(qt.dtype), _lib.stream_ptr(qt.device))
     _lib.check(rc, "afa_ago_rotate")
     return st.back(q_out), st.back(k_out)
+
+
+class AxisArguments(NamedTuple):
+    """Checked arguments of a rotation with several position axes."""
+    c: torch.Tensor          # (positions, dim / 2)
+    s: torch.Tensor
+    positions: torch.Tensor  # (axes, *shape) int32 or int64, any strides
+    sections: ctypes.Array
+
+
+def axis_arguments(rotary_params, positions, sections, dim, shape, device) -> AxisArguments:
+    """Tables, positions (axes, *shape) and channel pairs per axis of a rotation, checked, and on ``device`` if one
+    is given."""
+    if positions is None or sections is None:
+        raise ValueError("a rotation needs positions and sections")
+    sections = tuple(int(n) for n in sections)
+    if not 1 <= len(sections) <= 4:
+        raise ValueError("between one and four position axes are supported")
+    if any(n < 0 for n in sections) or sum(sections) > dim // 2:
+        raise ValueError(f"sections must be nonnegative and sum to at most {dim // 2}, got {sections}")
+    c, s = _extract_cs(rotary_params)
+    c, s = (torch.from_numpy(np.ascontiguousarray(x)) if isinstance(x, np.ndarray) else x for x in (c, s))
+    if not isinstance(c, torch.Tensor) or not isinstance(s, torch.Tensor) or c.dtype not in _TORCH_DTYPES.values() \
+            or s.dtype != c.dtype:
+        raise TypeError("the rotary tables must share a dtype: float32, bfloat16 or float64")
+    if c.shape != s.shape or c.ndim == 0 or c.shape[-1] != dim // 2 or c.numel() == 0:
+        raise ValueError(f"rotary tables must have shape (positions, {dim // 2}), got {tuple(c.shape)} and "
+                         f"{tuple(s.shape)}")
+    if c.requires_grad or s.requires_grad:
+        raise ValueError("the rotary tables have no gradient")
+    p = positions if isinstance(positions, torch.Tensor) else torch.as_tensor(np.asarray(positions))
+    if p.dtype not in (torch.int32, torch.int64):
+        raise TypeError("positions must be int32 or int64")
+    if tuple(p.shape) != (len(sections), *shape):
+        raise ValueError(f"positions must have shape {(len(sections), *shape)}, got {tuple(p.shape)}")
+    length = c.numel() // (dim // 2)
+    if not p.is_cuda and p.numel() and not (0 <= int(p.min()) and int(p.max()) < length):
+        raise ValueError(f"positions must lie in [0, {length}), the tables' rows")
+    if device is not None:
+        if any(x.is_cuda and x.device != device for x in (c, s, p)):
+            raise ValueError(f"tables and positions must be on {device}")
+        c, s, p = c.to(device), s.to(device), p.to(device)
+    c, s = (x.reshape(length, dim // 2).contiguous() for x in (c, s))
+    return AxisArguments(c, s, p, (ctypes.c_int * len(sections))(*sections))
+
+
+def _rotate_axes(q, k, axes: AxisArguments, backward: bool):
+    """One launch: q and k (or None) turned, backward the other way; contiguous results."""
+    token_major = q.ndim == 3
+    tensors = [t if t is None or t.stride(-1) == 1 else t.contiguous() for t in (q, k)]
+
+    def strides(t):  # batch, token, head
+        if t is None:
+            return None
+        return (ctypes.c_longlong * 3)(*((0, t.stride(0), t.stride(1)) if token_major else
+                                         (t.stride(0), t.stride(2), t.stride(1))))
+
+    outs = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in tensors]
+    batch, tokens = (1, q.shape[0]) if token_major else (q.shape[0], q.shape[2])
+    p = axes.positions
+    p_strides = (p.stride(0), 0 if p.ndim == 2 else p.stride(1), p.stride(-1))
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    with torch.cuda.device(q.device):
+        rc = _lib.load().afa_ago_rotate_axes(
+            ptr(tensors[0]), strides(tensors[0]), ptr(outs[0]), q.shape[1], ptr(tensors[1]), strides(tensors[1]),
+            ptr(outs[1]), 0 if k is None else k.shape[1], axes.c.data_ptr(), axes.s.data_ptr(),
+            _lib.dtype_code(axes.c.dtype), axes.c.shape[0], p.data_ptr(), (ctypes.c_longlong * 3)(*p_strides),
+            int(p.dtype == torch.int64), axes.sections, p.shape[0], int(token_major), batch, tokens, q.shape[-1],
+            int(backward), _lib.dtype_code(q.dtype), _lib.stream_ptr(q.device))
+    _lib.check(rc, "afa_ago_rotate_axes")
+    return outs[0], outs[1]
+
+
+class _RotateAxes(torch.autograd.Function):
+    """A rotation's gradient is the rotation the other way, which is differentiable again."""
+
+    @staticmethod
+    def forward(ctx, q, k, c, s, positions, sections, turn_back):
+        ctx.save_for_backward(c, s, positions)
+        ctx.sections, ctx.turn_back = sections, turn_back
+        qo, ko = _rotate_axes(q, k, AxisArguments(c, s, positions, sections), turn_back)
+        return qo if k is None else (qo, ko)
+
+    @staticmethod
+    def backward(ctx, gq, gk=None):
+        g = _RotateAxes.apply(gq, gk, *ctx.saved_tensors, ctx.sections, not ctx.turn_back)
+        return (*((g, None) if gk is None else g), None, None, None, None, None)
+
+
+def apply_ago_rotations_axes(q, k, rotary_params, positions, sections):
+    """AGO Cayley rotations with several position axes (time, height, width).
+
+    q (batch, heads, tokens, dim) or, packed, (tokens, heads, dim); k (or None)
+    the same with its own number of heads. ``sections`` gives each axis (at most
+    four) its channel pairs, in order: pair p of axis a at a token with
+    ``positions[a, ..., token]`` = m turns by row m of the tables, pairs behind
+    the last section stay as they are. ``positions``: (axes, batch, tokens),
+    (axes, tokens) for packed inputs or the same positions in every batch row,
+    int32 or int64; one the tables do not hold is an error on the host and gives
+    NaN on the device. ``rotary_params`` as in ``apply_ago_rotations``, (positions,
+    dim / 2). Unlike there the tables keep their dtype: the arithmetic is
+    float32 (float64 for float64 inputs) with one rounding, which a bfloat16
+    table would limit to 2^-9. Differentiable in q and k. Returns contiguous
+    (q_rot, k_rot).
+    """
+    if q.ndim not in (3, 4):
+        raise ValueError(f"q must have shape (batch, heads, tokens, dim) or (tokens, heads, dim), got {tuple(q.shape)}")
+    dim = q.shape[-1]
+    if dim % 2 != 0 or dim == 0:
+        raise ValueError(f"Feature dimension must be even, got {dim}")
+    head = 1
+    if k is not None and (k.ndim != q.ndim or [n for i, n in enumerate(k.shape) if i != head] !=
+                          [n for i, n in enumerate(q.shape) if i != head]):
+        raise ValueError(f"q and k must differ in their heads only, got {tuple(q.shape)} and {tuple(k.shape)}")
+    if q.shape[head] == 0 or (k is not None and k.shape[head] == 0):
+        raise ValueError("q and k need at least one head")
+    host_checks_float(*(t for t in (q, k) if t is not None))
+    if k is not None and k.dtype != q.dtype:
+        raise TypeError("q and k must share a dtype")
+    on_gpu = all(t is None or (isinstance(t, torch.Tensor) and t.is_cuda) for t in (q, k))
+    if on_gpu:
+        st, qt, kt = None, q, k
+        if k is not None and k.device != q.device:
+            raise ValueError(f"tensors on different devices: {q.device} and {k.device}")
+    else:
+        if any(isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k)):
+            raise ValueError("a differentiable rotation needs CUDA tensors")
+        axis_arguments(rotary_params, positions, sections, dim, _axis_shape(q, positions), None)
+        st = Staged(*(t for t in (q, k) if t is not None))
+        qt, kt = st.tensors[0], (st.tensors[1] if k is not None else None)
+    if qt.dtype not in _TORCH_DTYPES.values():
+        raise TypeError("q and k must be float32, bfloat16 or float64")
+    axes = axis_arguments(rotary_params, positions, sections, dim, _axis_shape(qt, positions), qt.device)
+    outs = _RotateAxes.apply(qt, kt, *axes, False)
+    outs = (outs, None) if kt is None else outs
+    return tuple(outs) if st is None else (st.back(outs[0]), st.back(outs[1]))
+
+
+def _axis_shape(q, positions):
+    """The shape positions must have behind their axes."""
+    if q.ndim == 3:
+        return (q.shape[0],)
+    if getattr(positions, "ndim", 3) == 2:
+        return (q.shape[2],)
+    return (q.shape[0], q.shape[2])

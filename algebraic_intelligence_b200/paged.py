@@ -1,0 +1,365 @@
+"""Serving from a paged key/value cache on B200 (no reference counterpart).
+
+A cache is a pair of tensors (pages, kv_heads, page_size, dim); request b keeps
+token j in page ``block_table[b, j // page_size]``, row ``j % page_size``.
+Lengths, tables and the stack of free pages live on the GPU, so a step needs no
+host copy and can be captured into a CUDA graph. One step of a server, whether
+its requests append a prompt, a token or a tree of drafted tokens:
+
+* ``paged_plan``    block tables, slot maps, positions and tree masks from the
+                    requests' lengths; refuses what does not fit
+* ``paged_append``  rotates the new queries and keys (several position axes,
+                    see ``apply_ago_rotations_axes``) and writes keys and
+                    values into the cache
+* ``afa_paged``     AFA of the new tokens over the cache: the math of
+                    ``pallas_afa_forward`` (src/kernels/pallas_afa.py:104-151)
+                    with the keys read through the block table
+* ``paged_commit``  moves the accepted path of a verified tree to its front;
+                    the next ``paged_plan`` takes back the other nodes' pages
+
+The tensors are CUDA tensors on one device; calls run on its current stream.
+The caches, the block table and the free stack are updated in place.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib
+from .ago import axis_arguments
+
+__all__ = ["PagedPlan", "paged_plan", "paged_append", "afa_paged", "paged_commit", "paged_workspace_bytes"]
+
+
+class PagedPlan(NamedTuple):
+    """What ``paged_plan`` returns (T = max_tokens, B requests)."""
+    slots: torch.Tensor        # (T,) int64: cache row page * page_size + offset, -1 behind the last token
+    rows: torch.Tensor         # (T,) int32: request, -1 behind the last token
+    positions: torch.Tensor    # (T,) int32: position in the request (a tree's: its length before + depth)
+    cu_tokens: torch.Tensor    # (B + 1,) int32: first new token of each request
+    seq_lens: torch.Tensor     # (B,) int32: lengths with the new tokens
+    page_counts: torch.Tensor  # (B,) int32: pages held
+    free_count: torch.Tensor   # (1,) int32: pages left on the stack
+    granted: torch.Tensor      # (B,) bool: False for a request whose tokens or pages did not fit
+    ancestors: Optional[torch.Tensor]  # (T, ceil(nodes / 32)) int32 words, with parents
+
+
+def _check_page_size(page_size) -> None:
+    if not isinstance(page_size, int) or page_size < 16 or page_size > 256 or page_size & (page_size - 1):
+        raise ValueError(f"page_size must be a power of two from 16 to 256, got {page_size}")
+
+
+def _ints(name, t, shape):
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+        raise TypeError(f"{name} must be an int32 tensor")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def _one_device(*tensors):
+    """The CUDA device that all tensors live on."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError("the paged operators need CUDA tensors")
+        if dev is not None and t.device != dev:
+            raise ValueError(f"tensors on different devices: {dev} and {t.device}")
+        dev = t.device
+    return dev
+
+
+def _on(dev):
+    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _no_gradient(what, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError(f"{what} has no gradient: call it under torch.no_grad()")
+
+
+def _caches(k_cache, v_cache, ndims=(4,)):
+    """Checks a pair of caches; returns (pages, kv_heads, page_size, dim)."""
+    if not isinstance(k_cache, torch.Tensor) or not isinstance(v_cache, torch.Tensor):
+        raise TypeError("the caches must be tensors")
+    if k_cache.ndim not in ndims or tuple(k_cache.shape) != tuple(v_cache.shape):
+        raise ValueError("k_cache and v_cache must have the same (pages, kv_heads, page_size, dim) shape, got "
+                         f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
+    if not k_cache.is_floating_point():
+        raise TypeError("expected a floating point array")
+    if k_cache.dtype != v_cache.dtype:
+        raise TypeError("k_cache and v_cache must share a dtype")
+    pages, heads, page_size, dim = k_cache.shape[-4:]
+    _check_page_size(page_size)
+    if k_cache.stride(-1) != 1 or v_cache.stride(-1) != 1:
+        raise ValueError("a cache row's channels must be contiguous")
+    return pages, heads, page_size, dim
+
+
+def _rows(t):
+    """A tensor whose last axis is contiguous."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _ll(*values):
+    return (ctypes.c_longlong * len(values))(*values)
+
+
+def paged_plan(block_table, page_counts, seq_lens, new_lens, free_pages, free_count, page_size: int, max_tokens: int,
+               parents=None) -> PagedPlan:
+    """Block tables, slot maps and tree masks of one step, from the requests' lengths.
+
+    block_table (B, columns), page_counts (B,): the pages each request holds;
+    seq_lens (B,): its tokens; new_lens (B,): tokens it appends (below 0 counts
+    as 0); free_pages (N,), free_count (1,): the stack of free pages. All int32
+    on the GPU. With need = ceil((seq_lens + new_lens) / page_size), pages a
+    request holds behind ``need`` (it ended, or drafted tokens were rejected)
+    are released onto the stack in request order; then the requests that need
+    more take them from its top, in request order. ``block_table`` and
+    ``free_pages`` are updated in place; lengths and counts come back in new
+    tensors, so a call with the same inputs gives the same step.
+
+    A request is refused (``granted`` False; it keeps what it holds and gets no
+    tokens) when its row of the table is too short, when the tokens asked for
+    up to and with it pass ``max_tokens``, or when the pages run out.
+
+    ``parents`` (B, nodes <= 256) int32: each request's new tokens form a tree;
+    ``parents[b, i]`` in [0, i) is token i's parent, any other value makes it a
+    root. Positions are then seq_len + depth, and ``ancestors`` holds the words
+    ``afa_paged`` takes.
+    """
+    if not isinstance(block_table, torch.Tensor) or block_table.dtype != torch.int32:
+        raise TypeError("block_table must be an int32 tensor")
+    if block_table.ndim != 2 or not block_table.is_contiguous() or block_table.numel() == 0:
+        raise ValueError("block_table must be a contiguous (batch, columns) tensor")
+    b, cols = block_table.shape
+    if b > 4096:
+        raise ValueError("paged_plan: batch must be in [1, 4096]")
+    _check_page_size(page_size)
+    if not isinstance(max_tokens, int) or max_tokens < 0:
+        raise ValueError("max_tokens must be a nonnegative integer")
+    for name, t in (("page_counts", page_counts), ("seq_lens", seq_lens), ("new_lens", new_lens)):
+        _ints(name, t, (b,))
+    _ints("free_count", free_count, (1,))
+    if not isinstance(free_pages, torch.Tensor) or free_pages.dtype != torch.int32:
+        raise TypeError("free_pages must be an int32 tensor")
+    if free_pages.ndim != 1 or not free_pages.is_contiguous() or free_pages.numel() == 0:
+        raise ValueError("free_pages must be a contiguous one-dimensional tensor")
+    nodes = 0
+    if parents is not None:
+        if not isinstance(parents, torch.Tensor) or parents.ndim != 2:
+            raise ValueError("parents must have shape (batch, nodes)")
+        nodes = parents.shape[1]
+        _ints("parents", parents, (b, nodes))
+        if not 1 <= nodes <= 256:
+            raise ValueError("a tree may have at most 256 nodes")
+    dev = _one_device(block_table, page_counts, seq_lens, new_lens, free_pages, free_count, parents)
+    page_counts, seq_lens, new_lens = page_counts.contiguous(), seq_lens.contiguous(), new_lens.contiguous()
+    parents = parents.contiguous() if parents is not None else None
+    slots = torch.empty(max_tokens, dtype=torch.int64, device=dev)
+    per_token = torch.empty((2, max_tokens), dtype=torch.int32, device=dev)
+    per_request = torch.empty(3 * b + 2, dtype=torch.int32, device=dev)
+    cu, lens_out, held_out, free_out = per_request.split((b + 1, b, b, 1))
+    rows, positions = per_token[0], per_token[1]
+    granted = torch.empty(b, dtype=torch.bool, device=dev)
+    ancestors = torch.empty((max_tokens, (nodes + 31) // 32), dtype=torch.int32, device=dev) if nodes else None
+    with _on(dev):
+        rc = _lib.load().afa_paged_plan(
+            block_table.data_ptr(), page_counts.data_ptr(), seq_lens.data_ptr(), new_lens.data_ptr(),
+            free_pages.data_ptr(), free_count.data_ptr(), parents.data_ptr() if nodes else None, slots.data_ptr(),
+            rows.data_ptr(), positions.data_ptr(), cu.data_ptr(), lens_out.data_ptr(), held_out.data_ptr(),
+            free_out.data_ptr(), granted.data_ptr(), ancestors.data_ptr() if nodes else None, b, cols, page_size,
+            free_pages.numel(), max_tokens, nodes, _lib.stream_ptr(dev))
+    _lib.check(rc, "afa_paged_plan")
+    return PagedPlan(slots, rows, positions, cu, lens_out, held_out, free_out, granted, ancestors)
+
+
+def paged_append(k, v, k_cache, v_cache, slots, q=None, rotary_params=None, positions=None, sections=None):
+    """Writes new keys and values into a paged cache, rotating on the way.
+
+    k, v (tokens, kv_heads, dim) go to cache rows ``slots`` (tokens,) int64 (a
+    ``PagedPlan``'s); a slot outside the cache, such as a padded token's -1, is
+    skipped, and slots inside it are distinct. With ``rotary_params``,
+    ``positions`` (axes, tokens) and ``sections`` as in
+    ``apply_ago_rotations_axes`` the keys are rotated, and so is ``q`` (tokens,
+    heads, dim), which comes back; without q the result is None. The caches may
+    be strided views (such as a (pages, page_size, heads, dim) cache
+    transposed).
+    """
+    pages, heads, page_size, dim = _caches(k_cache, v_cache)
+    if k.ndim != 3 or tuple(k.shape) != tuple(v.shape) or tuple(k.shape[1:]) != (heads, dim):
+        raise ValueError(f"k and v must have shape (tokens, {heads}, {dim}), got {tuple(k.shape)} and "
+                         f"{tuple(v.shape)}")
+    tokens = k.shape[0]
+    if q is not None and (q.ndim != 3 or q.shape[0] != tokens or q.shape[2] != dim or q.shape[1] == 0):
+        raise ValueError(f"q must have shape ({tokens}, heads, {dim}), got {tuple(q.shape)}")
+    if any(t is not None and t.dtype != k_cache.dtype for t in (k, v, q)):
+        raise TypeError("k, v, q and the caches must share a dtype")
+    if k_cache.dtype == torch.float16:
+        raise TypeError("float16 is not supported; use bfloat16 or float32")
+    if not isinstance(slots, torch.Tensor) or slots.dtype not in (torch.int64, torch.int32):
+        raise TypeError("slots must be an int64 tensor")
+    if tuple(slots.shape) != (tokens,):
+        raise ValueError(f"slots must have shape ({tokens},), got {tuple(slots.shape)}")
+    if dim % 2 != 0:
+        raise ValueError(f"Feature dimension must be even, got {dim}")
+    if rotary_params is None and (q is not None or positions is not None or sections is not None):
+        raise ValueError("q, positions and sections go with rotary_params")
+    _no_gradient("paged_append", k, v, q)
+    dev = _one_device(k_cache, v_cache, k, v, q, slots)
+    axes = axis_arguments(rotary_params, positions, sections, dim, (tokens,), dev) if rotary_params is not None \
+        else None
+    k, v = _rows(k), _rows(v)
+    slots = slots.to(torch.int64).contiguous()
+    out = None
+    if q is not None:
+        q = _rows(q)
+        out = torch.empty((tokens, q.shape[1], dim), dtype=q.dtype, device=dev)
+    if axes is not None:
+        p = axes.positions
+        pos = (axes.c.data_ptr(), axes.s.data_ptr(), _lib.dtype_code(axes.c.dtype), axes.c.shape[0], p.data_ptr(),
+               _ll(p.stride(0), p.stride(1)), int(p.dtype == torch.int64), axes.sections, p.shape[0])
+    else:
+        pos = (None, None, 0, 0, None, None, 0, None, 0)
+    with _on(dev):
+        rc = _lib.load().afa_paged_append(
+            k.data_ptr(), _ll(k.stride(0), k.stride(1)), v.data_ptr(), _ll(v.stride(0), v.stride(1)),
+            k_cache.data_ptr(), _ll(*k_cache.stride()[:3]), v_cache.data_ptr(), _ll(*v_cache.stride()[:3]),
+            slots.data_ptr(), None if q is None else q.data_ptr(),
+            None if q is None else _ll(q.stride(0), q.stride(1)), None if out is None else out.data_ptr(),
+            0 if q is None else q.shape[1], *pos, tokens, heads, dim, pages, page_size,
+            _lib.dtype_code(k_cache.dtype), _lib.stream_ptr(dev))
+    _lib.check(rc, "afa_paged_append")
+    return out
+
+
+def paged_workspace_bytes(tokens: int, q_heads: int, kv_heads: int, head_dim: int, dtype=torch.bfloat16) -> int:
+    """Scratch bytes ``afa_paged`` needs for this shape."""
+    return int(_lib.load().afa_paged_workspace_bytes(tokens, q_heads, kv_heads, head_dim, _lib.dtype_code(dtype)))
+
+
+def afa_paged(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, ancestors=None, sink_omega: float = 0.5,
+              return_denominator: bool = False, out: Optional[torch.Tensor] = None,
+              workspace: Optional[torch.Tensor] = None):
+    """AFA of new tokens over a paged cache: single tokens, prompt chunks, drafted trees.
+
+    q (tokens, heads, dim): the requests' new tokens one after the other,
+    request b's from ``cu_tokens[b]`` to ``cu_tokens[b + 1]``; heads a multiple
+    of the cache's, head h reading key head h // (heads / kv_heads).
+    ``seq_lens`` (B,) counts a request's keys, its n new tokens (already in the
+    cache) included. A new token sees the seq_len - n keys before them, and of
+    the new ones those up to itself or, with ``ancestors`` (tokens, words) int32
+    (bit j of word j // 32: new token j of its request), those whose bit is set.
+    Keys whose table entry names no page of the cache are not seen; a row that
+    sees no key gives output 0 and d_total = sink_omega. Cached rows of a
+    request must be finite; what lies behind its last token does not matter.
+
+    Returns out (tokens, heads, dim), with ``return_denominator`` also d_total
+    (tokens, heads) in the accumulation dtype. Rows of q behind the last request
+    are not computed: with ``out`` given they are left as they were, otherwise
+    their contents are unspecified. ``workspace`` (see
+    ``paged_workspace_bytes``) is overwritten; calls that may overlap need one
+    each. bfloat16 with dim 64 or 128 runs on the tensor cores.
+    """
+    if not 0 <= sink_omega < float("inf"):
+        raise ValueError("sink_omega must be finite and nonnegative")
+    pages, kv_heads, page_size, dim = _caches(k_cache, v_cache)
+    if not isinstance(q, torch.Tensor) or not q.is_floating_point():
+        raise TypeError("expected a floating point array")
+    if q.ndim != 3 or q.shape[2] != dim or q.shape[1] == 0 or q.shape[1] % kv_heads != 0:
+        raise ValueError(f"q must have shape (tokens, heads, {dim}) with heads a multiple of {kv_heads}, got "
+                         f"{tuple(q.shape)}")
+    if q.dtype != k_cache.dtype:
+        raise TypeError("q and the caches must share a dtype")
+    code = _lib.dtype_code(q.dtype)
+    if code == _lib.AFA_F16:
+        raise TypeError("float16 is not supported: rho(s)^8 overflows float16 for s > 2.4; use bfloat16 or float32")
+    tokens, heads, _ = q.shape
+    if not isinstance(block_table, torch.Tensor) or block_table.dtype != torch.int32:
+        raise TypeError("block_table must be an int32 tensor")
+    if block_table.ndim != 2 or block_table.numel() == 0:
+        raise ValueError("block_table must have shape (batch, columns)")
+    b, cols = block_table.shape
+    _ints("seq_lens", seq_lens, (b,))
+    _ints("cu_tokens", cu_tokens, (b + 1,))
+    words = 0
+    if ancestors is not None:
+        if not isinstance(ancestors, torch.Tensor) or ancestors.dtype != torch.int32:
+            raise TypeError("ancestors must be an int32 tensor")
+        if ancestors.ndim != 2 or ancestors.shape[0] != tokens or ancestors.shape[1] == 0:
+            raise ValueError(f"ancestors must have shape ({tokens}, words), got {tuple(ancestors.shape)}")
+        words = ancestors.shape[1]
+        ancestors = _rows(ancestors)
+    if out is not None and (tuple(out.shape) != tuple(q.shape) or out.dtype != q.dtype or not out.is_contiguous()):
+        raise ValueError("out must be a contiguous tensor of q's shape and dtype")
+    _no_gradient("afa_paged", q, k_cache, v_cache)
+    dev = _one_device(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, ancestors, out, workspace)
+    q, block_table = _rows(q), _rows(block_table)
+    seq_lens, cu_tokens = seq_lens.contiguous(), cu_tokens.contiguous()
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=dev)
+    den = torch.empty((tokens, heads), dtype=_lib.accum_dtype(q.dtype), device=dev) if return_denominator else None
+    lib = _lib.load()
+    need = lib.afa_paged_workspace_bytes(tokens, heads, kv_heads, dim, code)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    elif not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < need:
+        raise ValueError(f"workspace must be a contiguous tensor of at least {need} bytes")
+    with _on(dev):
+        rc = lib.afa_paged(
+            q.data_ptr(), _ll(q.stride(0), q.stride(1)), k_cache.data_ptr(), v_cache.data_ptr(),
+            _ll(*k_cache.stride()[:3]), _ll(*v_cache.stride()[:3]), out.data_ptr(),
+            None if den is None else den.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+            seq_lens.data_ptr(), cu_tokens.data_ptr(), ancestors.data_ptr() if words else None,
+            ancestors.stride(0) if words else 0, words, b, tokens, heads, kv_heads, dim, cols, page_size, pages, code,
+            float(sink_omega), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+            _lib.stream_ptr(dev))
+    _lib.check(rc, "afa_paged")
+    return (out, den) if return_denominator else out
+
+
+def paged_commit(k_cache, v_cache, block_table, base_lens, seq_lens, accepted) -> torch.Tensor:
+    """Moves the accepted path of each request's drafted tree to its front.
+
+    ``base_lens`` (B,): tokens before the tree; ``seq_lens`` (B,): with it;
+    ``accepted`` (B, path <= 256): the accepted nodes from the root on, -1
+    behind the last. Cache row base + i becomes row base + accepted[i] for the
+    longest prefix of ``accepted`` that ascends strictly, lies in the tree and
+    whose pages are in the cache. The caches may hold several layers, (layers,
+    pages, kv_heads, page_size, dim). Returns the lengths base + accepted (B,)
+    int32, the next ``paged_plan``'s ``seq_lens``.
+    """
+    pages, heads, page_size, dim = _caches(k_cache, v_cache, (4, 5))
+    if k_cache.dtype == torch.float16:
+        raise TypeError("float16 is not supported; use bfloat16 or float32")
+    if not isinstance(block_table, torch.Tensor) or block_table.dtype != torch.int32:
+        raise TypeError("block_table must be an int32 tensor")
+    if block_table.ndim != 2 or block_table.numel() == 0:
+        raise ValueError("block_table must have shape (batch, columns)")
+    b, cols = block_table.shape
+    _ints("base_lens", base_lens, (b,))
+    _ints("seq_lens", seq_lens, (b,))
+    if not isinstance(accepted, torch.Tensor) or accepted.ndim != 2:
+        raise ValueError("accepted must have shape (batch, path)")
+    path = accepted.shape[1]
+    _ints("accepted", accepted, (b, path))
+    if path > 256:
+        raise ValueError("an accepted path may have at most 256 tokens")
+    dev = _one_device(k_cache, v_cache, block_table, base_lens, seq_lens, accepted)
+    block_table, accepted = _rows(block_table), _rows(accepted)
+    base_lens, seq_lens = base_lens.contiguous(), seq_lens.contiguous()
+    lens = torch.empty(b, dtype=torch.int32, device=dev)
+    layers = k_cache.shape[0] if k_cache.ndim == 5 else 1
+    strides = [(0, *t.stride()[:3]) if t.ndim == 4 else t.stride()[:4] for t in (k_cache, v_cache)]
+    with _on(dev):
+        rc = _lib.load().afa_paged_commit(
+            k_cache.data_ptr(), _ll(*strides[0]), v_cache.data_ptr(), _ll(*strides[1]), block_table.data_ptr(),
+            block_table.stride(0), base_lens.data_ptr(), seq_lens.data_ptr(), accepted.data_ptr(),
+            accepted.stride(0) if path else 0, lens.data_ptr(), b, path, layers, heads, dim, cols, pages, page_size,
+            _lib.dtype_code(k_cache.dtype), _lib.stream_ptr(dev))
+    _lib.check(rc, "afa_paged_commit")
+    return lens

@@ -19,6 +19,11 @@
  *                            of pallas_afa (:555-615)
  *   afa_ago_table         <- build_cayley_rotary_matrix (src/attention.py:156-207)
  *   afa_ago_rotate        <- apply_ago_rotations (src/attention.py:210-240)
+ *   afa_ago_rotate_axes   <- no reference counterpart: the same with several
+ *                            position axes, forward and gradient
+ *   afa_paged_plan, afa_paged_append, afa_paged, afa_paged_commit
+ *                         <- no reference counterpart: serving from a paged
+ *                            cache, trees of drafted tokens included
  *   afa_decode            <- no reference counterpart: exact AFA for one query
  *                            token over a KV cache (pallas_afa_forward with Lq=1)
  *   algebraic_softmax_fwd <- algebraic_softmax   (src/attention.py:88-91, :59-67)
@@ -210,6 +215,28 @@ AFA_API int afa_ago_rotate(const void* q, const void* k, void* q_out, void* k_ou
                            void* stream);
 
 /*
+ * afa_ago_rotate_axes  the rotation with several position axes (time, height,
+ *                 width; no reference counterpart): channel pairs
+ *                 [sum sections[< a], + sections[a]) turn by row
+ *                 positions[a][b][t] of the tables, pairs behind the last
+ *                 section stay as they are. q (batch, tokens, q_heads, dim) and
+ *                 k (k_heads; may be NULL) by strides (batch, token, head);
+ *                 outputs contiguous, (batch, tokens, heads, dim) when
+ *                 token_major, else (batch, heads, tokens, dim). positions:
+ *                 int32, or int64 when positions_64, strides (axis, batch,
+ *                 token); a position the tables (table_len, dim / 2) do not
+ *                 hold makes its pairs NaN. backward: turns the other way, the
+ *                 gradient. At most four axes. Arithmetic in float32 (float64
+ *                 for AFA_F64), one rounding.
+ */
+AFA_API int afa_ago_rotate_axes(const void* q, const long long* q_strides, void* q_out, int q_heads, const void* k,
+                                const long long* k_strides, void* k_out, int k_heads, const void* c, const void* s,
+                                int table_dtype, int table_len, const void* positions,
+                                const long long* position_strides, int positions_64, const int* sections, int axes,
+                                int token_major, int batch, int tokens, int dim, int backward, int dtype,
+                                void* stream);
+
+/*
  * Decode step (no reference counterpart; the math of pallas_afa_forward with a
  * single query row, non-causal).
  *   q           (B, H, D) -- one token per (batch, head)
@@ -246,6 +273,100 @@ AFA_API size_t afa_decode_workspace_bytes(int B, int H, int Lkv, int D);
 AFA_API int afa_decode_noalloc(const void* q, const void* k_cache, const void* v_cache, void* out, void* d_total,
                                int B, int H, int Lkv, int D, int dtype, float sink_omega, const int* kv_lens,
                                int kv_len, void* stream);
+
+/*
+ * Serving from a paged key/value cache (no reference counterpart). A cache is
+ * (pages, kv_heads, page_size, D) with page_size a power of two from 16 to 256;
+ * request b's token j lies in page block_table[b][j / page_size], row
+ * j % page_size. All lengths, tables and slots are device memory: a step needs
+ * no host copy and can be captured. Strides are in elements; a row's D elements
+ * are contiguous.
+ *
+ * afa_paged_plan  Block tables, slot maps and tree masks of one step from the
+ *                 requests' lengths. Request b holds the pages
+ *                 block_table[b][0 .. page_counts[b]) and seq_lens[b] tokens
+ *                 and appends new_lens[b] (below 0 counts as 0). With
+ *                 need = ceil((seq_lens + new_lens) / page_size), pages behind
+ *                 `need` are released: in request order they join the top of
+ *                 the stack free_pages[0 .. free_count). Then the requests that
+ *                 need more take them from the top, in request order. A request
+ *                 is refused, keeping what it holds, when its row of the table
+ *                 (table_cols) or, with parents, a tree of `nodes` is too
+ *                 small for it, when the tokens asked for up to and with it
+ *                 pass max_tokens, or when the pages do.
+ *   block_table   (batch, table_cols) int32, entries behind the pages held are
+ *                 written; free_pages (num_free) int32, the entries behind
+ *                 what stays are written. The rest of both is left as it is.
+ *   parents       optional (batch, nodes) int32: the new tokens of a request
+ *                 form a tree; parents[b][i] in [0, i) is token i's parent,
+ *                 any other value makes it a root.
+ *   slots, rows, positions  (max_tokens): cache row, request and position of
+ *                 each new token, requests one after the other; behind the
+ *                 last -1, -1 and 0. A tree's positions are seq_len + depth.
+ *   cu_tokens     (batch + 1): first new token of each request.
+ *   seq_lens_out, page_counts_out, free_count_out, granted  the state after the
+ *                 step, in arrays other than its inputs.
+ *   ancestors     (max_tokens, ceil(nodes / 32)) 32-bit words: bit j of a
+ *                 token's words is set when new token j is on its path to the
+ *                 root (itself among them).
+ *   batch at most 4096, nodes at most 256.
+ *
+ * afa_paged_append  k, v (tokens, kv_heads, D) into rows slots[token] of the
+ *                 caches (slots outside the cache are skipped; distinct slots
+ *                 are the caller's care). With rotary tables (c != NULL) k is
+ *                 rotated on the way, and q (tokens, q_heads, D), if given,
+ *                 into q_out (contiguous). Strides: k, v, q (token, head);
+ *                 caches (page, head, row); positions (axis, token).
+ *
+ * afa_paged       AFA of the new tokens (q: tokens, q_heads, D; the requests'
+ *                 tokens from cu_tokens[b] on) over the cache. seq_lens counts
+ *                 a request's keys, its n new tokens included. Row t sees the
+ *                 seq_len - n keys before the new tokens, and of those, up to
+ *                 itself (ancestors NULL) or the ones whose bit in its ancestor
+ *                 words is set. Keys whose table entry names no page of the
+ *                 cache are not seen. Query heads [h q_heads / kv_heads, ...)
+ *                 share key head h. out (tokens, q_heads, D) and d_total
+ *                 (tokens, q_heads; may be NULL) are contiguous; a row that
+ *                 sees no key gives 0 and sink_omega, rows of no request are
+ *                 not written. Cached rows of a request must be finite; what
+ *                 lies behind its last token does not matter.
+ *                 AFA_F32, AFA_BF16, AFA_F64; D at most 256.
+ *   workspace     afa_paged_workspace_bytes bytes, overwritten by each call;
+ *                 calls that overlap need one each.
+ *
+ * afa_paged_commit  After a tree was verified: cache row base_lens[b] + i
+ *                 becomes row base_lens[b] + accepted[b][i], for the longest
+ *                 prefix of `accepted` (batch, path; at most 256) that
+ *                 ascends strictly from 0 or more, lies below seq_lens[b] and
+ *                 has its pages in the cache. lens_out[b] = base_lens[b] + its
+ *                 length. Caches may hold several layers: strides (layer, page,
+ *                 head, row).
+ */
+AFA_API int afa_paged_plan(int* block_table, const int* page_counts, const int* seq_lens, const int* new_lens,
+                           int* free_pages, const int* free_count, const int* parents, long long* slots, int* rows,
+                           int* positions, int* cu_tokens, int* seq_lens_out, int* page_counts_out,
+                           int* free_count_out, unsigned char* granted, void* ancestors, int batch, int table_cols,
+                           int page_size, int num_free, int max_tokens, int nodes, void* stream);
+AFA_API int afa_paged_append(const void* k, const long long* k_strides, const void* v, const long long* v_strides,
+                             void* k_cache, const long long* k_cache_strides, void* v_cache,
+                             const long long* v_cache_strides, const long long* slots, const void* q,
+                             const long long* q_strides, void* q_out, int q_heads, const void* c, const void* s,
+                             int table_dtype, int table_len, const void* positions,
+                             const long long* position_strides, int positions_64, const int* sections, int axes,
+                             int tokens, int kv_heads, int dim, int num_pages, int page_size, int dtype,
+                             void* stream);
+AFA_API int afa_paged(const void* q, const long long* q_strides, const void* k_cache, const void* v_cache,
+                      const long long* k_strides, const long long* v_strides, void* out, void* d_total,
+                      const int* block_table, long long table_stride, const int* seq_lens, const int* cu_tokens,
+                      const void* ancestors, long long ancestors_stride, int ancestor_words, int batch, int tokens,
+                      int q_heads, int kv_heads, int D, int table_cols, int page_size, int num_pages, int dtype,
+                      float sink_omega, void* workspace, size_t workspace_bytes, void* stream);
+AFA_API size_t afa_paged_workspace_bytes(int tokens, int q_heads, int kv_heads, int D, int dtype);
+AFA_API int afa_paged_commit(void* k_cache, const long long* k_strides, void* v_cache, const long long* v_strides,
+                             const int* block_table, long long table_stride, const int* base_lens,
+                             const int* seq_lens, const int* accepted, long long accepted_stride, int* lens_out,
+                             int batch, int path, int layers, int kv_heads, int dim, int table_cols, int num_pages,
+                             int page_size, int dtype, void* stream);
 
 /*
  * algebraic_softmax (src/attention.py:88-91): rows x cols, last axis
