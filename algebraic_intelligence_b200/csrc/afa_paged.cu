@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(kSimtThreads) afa_paged_simt_kernel(const __gr
   A* dtot = static_cast<A*>(a.dtot);
   const A scale = sizeof(A) == 8 ? static_cast<A>(a.scale_d) : static_cast<A>(a.scale);
   const A sink = sizeof(A) == 8 ? static_cast<A>(a.sink_d) : static_cast<A>(a.sink);
-  A* frag = static_cast<A*>(a.frag) + static_cast<long long>(blockIdx.x) * 2 * a.unit_rows * (D + 1);
+  A* frag = static_cast<A*>(a.frag) + static_cast<long long>(blockIdx.x) * 2 * a.frag_rows * (D + 1);
 
   PagedWalk walk;
   walk.init(a, paged_share<kSimtThreads>(a, share_sm));
@@ -184,13 +184,13 @@ __global__ void __launch_bounds__(kSimtThreads) afa_paged_simt_kernel(const __gr
         }
         if (tx == 0 && dtot) dtot[orow] = denom;
       } else {
-        A* f = frag + static_cast<long long>(paged_frag_slot(p)) * a.unit_rows * (D + 1);
+        A* f = frag + static_cast<long long>(paged_frag_slot(p)) * a.frag_rows * (D + 1);
 #pragma unroll
         for (int j = 0; j < OC; ++j) {
           const int c = tx + 16 * j;
           if (c < D) f[r * D + c] = o[i][j];
         }
-        if (tx == 0) f[a.unit_rows * D + r] = rs[i];
+        if (tx == 0) f[a.frag_rows * D + r] = rs[i];
       }
     }
   }
@@ -210,13 +210,13 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constan
   const PagedReq req = paged_req(a, b);
   const long long row0 = static_cast<long long>(u) * a.unit_rows;
   const int rows = static_cast<int>(min(static_cast<long long>(a.unit_rows), static_cast<long long>(req.n) * a.G - row0));
-  const long long size = static_cast<long long>(a.unit_rows) * (D + 1);
+  const long long size = static_cast<long long>(a.frag_rows) * (D + 1);
   const A* frag = static_cast<const A*>(a.frag);
   const A sink = sizeof(A) == 8 ? static_cast<A>(a.sink_d) : static_cast<A>(a.sink);
   const int lane = threadIdx.x & 31;
   for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.y * 8) {
-    A den = frag[(2LL * c + 1) * size + static_cast<long long>(a.unit_rows) * D + r];
-    for (int x = c + 1; x <= last; ++x) den += frag[2LL * x * size + static_cast<long long>(a.unit_rows) * D + r];
+    A den = frag[(2LL * c + 1) * size + static_cast<long long>(a.frag_rows) * D + r];
+    for (int x = c + 1; x <= last; ++x) den += frag[2LL * x * size + static_cast<long long>(a.frag_rows) * D + r];
     den += sink;
     const long long row = row0 + r, tok = req.tok0 + row / a.G;
     const long long orow = tok * a.Hkv * a.G + static_cast<long long>(h) * a.G + row % a.G;
@@ -262,7 +262,7 @@ cudaError_t launch_simt_type(const PagedArgs& a, int ctas, cudaStream_t stream) 
 template <typename T, typename A>
 cudaError_t launch_combine(const PagedArgs& a, int ctas, cudaStream_t stream) {
   if (ctas < 2) return cudaSuccess;
-  const dim3 grid(ctas - 1, (a.unit_rows + 63) / 64);
+  const dim3 grid(ctas - 1, (a.frag_rows + 63) / 64);
   paged_combine_kernel<T, A><<<grid, 256, 0, stream>>>(a, ctas);
   return cudaGetLastError();
 }
@@ -280,17 +280,20 @@ int sm_count() {
 constexpr int kMaxPagedCtas = 148;
 
 // Query rows per work unit and the workspace layout: meta, then fragments.
-int unit_rows_of(int dtype, int G, int D) {
-  const bool tc = dtype == kBF16 && (D == 64 || D == 128) && G <= 128;
-  (void)tc;
-  return kSimtRows;
+// Sized for the tensor-core kernel's units where it may run.
+int max_unit_rows(int dtype, int G, int D) {
+  return dtype == kBF16 && (D == 64 || D == 128) && G <= 128 ? paged_tc_unit_rows(G) : kSimtRows;
+}
+// A multiple of four, so that fragments start on 16 bytes whatever D is.
+int frag_rows_of(int unit_rows, int T, int G) {
+  const long long all = static_cast<long long>(T) * G;
+  return ((all < unit_rows ? static_cast<int>(all) : unit_rows) + 3) / 4 * 4;
 }
 constexpr size_t kMetaBytes = (static_cast<size_t>(kMaxPagedCtas) * 4 * sizeof(int) + 255) / 256 * 256;
 
 size_t workspace_bytes(int T, int Hq, int Hkv, int D, int dtype) {
   const size_t acc = dtype == kF64 ? 8 : 4;
-  size_t rows = unit_rows_of(dtype, Hq / Hkv, D);
-  (void)T;
+  const size_t rows = frag_rows_of(max_unit_rows(dtype, Hq / Hkv, D), T, Hq / Hkv);
   return kMetaBytes + static_cast<size_t>(kMaxPagedCtas) * 2 * rows * (static_cast<size_t>(D) + 1) * acc;
 }
 
@@ -365,7 +368,6 @@ extern "C" int afa_paged(const void* q, const long long* q_strides, const void* 
   a.table_cols = table_cols;
   a.page_shift = __builtin_ctz(static_cast<unsigned>(page_size));
   a.num_pages = num_pages;
-  a.unit_rows = unit_rows_of(dtype, a.G, D);
   a.scale_d = 1.0 / std::sqrt(static_cast<double>(D));
   a.scale = static_cast<float>(a.scale_d);
   a.sink_d = static_cast<double>(sink_omega);
@@ -377,8 +379,14 @@ extern "C" int afa_paged(const void* q, const long long* q_strides, const void* 
   if (!a.status || ctas <= 0) return set_last_error(AFA_ERR_CUDA, "afa_paged: device set-up failed");
   if (ctas > kMaxPagedCtas) ctas = kMaxPagedCtas;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool tc = paged_tc_supported(a, dtype);
+  a.unit_rows = tc ? paged_tc_unit_rows(a.G) : kSimtRows;
+  a.frag_rows = frag_rows_of(a.unit_rows, tokens, a.G);
+  const char* detail = "";
   cudaError_t e;
-  switch (dtype) {
+  if (tc) {
+    e = launch_paged_tc(a, ctas, st, &detail);
+  } else switch (dtype) {
     case kF64: e = launch_simt_type<double, double>(a, ctas, st); break;
     case kF32: e = launch_simt_type<float, float>(a, ctas, st); break;
     default: e = launch_simt_type<__nv_bfloat16, float>(a, ctas, st); break;
@@ -392,7 +400,7 @@ extern "C" int afa_paged(const void* q, const long long* q_strides, const void* 
   }
   if (e != cudaSuccess) {
     char msg[200];
-    snprintf(msg, sizeof(msg), "afa_paged launch: %s", cudaGetErrorString(e));
+    snprintf(msg, sizeof(msg), "afa_paged launch: %s %s", cudaGetErrorString(e), detail);
     return set_last_error(AFA_ERR_CUDA, msg);
   }
   return AFA_OK;

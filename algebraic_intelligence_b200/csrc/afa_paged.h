@@ -24,10 +24,11 @@ struct PagedArgs {
   long long q_st, q_sh, k_sp, k_sh, k_sr, v_sp, v_sh, v_sr, table_ld, anc_ld;
   int B, T, Hkv, G, D, table_cols, page_shift, num_pages, words;
   int unit_rows;            // query rows (token, head of the group) per work unit
+  int frag_rows;            // rows of a fragment: unit_rows, or all rows there can be if fewer
   double scale_d, sink_d;
   float scale, sink;
   int* meta;                // workspace: 4 ints per CTA (see PagedPiece)
-  void* frag;               // workspace: two fragments of unit_rows * (D + 1) sums per CTA
+  void* frag;               // workspace: two fragments of frag_rows * (D + 1) sums per CTA
   int* status;
 };
 
