@@ -305,7 +305,6 @@ __global__ void __launch_bounds__(576, 1)
             umma_commit(s_full + i);
             umma_commit(kv_empty + u % C::NSLOT);
             if (i + 1 == n) umma_commit(q_empty);
-            if (i == 1 && n == 2) umma_commit(q_empty);
           }
         }
         for (int i = 0; ok && i < n; ++i) {

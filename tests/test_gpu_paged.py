@@ -415,6 +415,24 @@ def test_attention_repeats_and_streams(dtype, dim):
     assert all(torch.equal(g, want) for g in got)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new,group", [(1, 4), (30, 4), (50, 4)])
+def test_attention_pieces_of_every_length(dim, new, group):
+    """Many requests of every number of key tiles, so that shares begin and end units of one, two and more tiles,
+    launched back to back: the same bits as one request at a time, and no wait runs out."""
+    lens = [max(new, 128 * (i % 9) + 1 + 37 * i % 128) for i in range(60)]
+    b = Batch(10, [new] * 60, lens, 3, group, dim, 128, BF)
+    args = b.args()
+    outs = [afa.afa_paged(*args) for _ in range(40)]
+    assert _lib.device_status(outs[0].device) == 0
+    assert all(torch.equal(o, outs[0]) for o in outs)
+    q, k, v, table, slens, cu, _ = args
+    for i in range(0, 60, 7):
+        one = afa.afa_paged(q[i * new:(i + 1) * new], k, v, table[i:i + 1], slens[i:i + 1], i32([0, new]))
+        # other splits add the float32 sums in another order, then both round to bfloat16 once
+        assert orc.rel_err(host(outs[0][i * new:(i + 1) * new]), host(one)) <= 2.0 ** -7
+
+
 def test_step_captured_and_replayed_with_other_lengths():
     """Plan, append and attention in one graph: the lengths it was captured with do not matter."""
     rng = np.random.default_rng(8)
