@@ -57,6 +57,7 @@ __global__ void __launch_bounds__(kSimtThreads) afa_paged_simt_kernel(const __gr
   const A sink = sizeof(A) == 8 ? static_cast<A>(a.sink_d) : static_cast<A>(a.sink);
   A* frag = static_cast<A*>(a.frag) + static_cast<long long>(blockIdx.x) * 2 * a.frag_rows * (D + 1);
 
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // see paged_combine_kernel
   PagedWalk walk;
   walk.init(a, paged_share<kSimtThreads>(a, share_sm));
   if (tid == 0) paged_meta_clear(a.meta);
@@ -197,34 +198,64 @@ __global__ void __launch_bounds__(kSimtThreads) afa_paged_simt_kernel(const __gr
 }
 
 // Adds the fragments of the unit that CTA blockIdx.x of the attention kernel
-// began and did not end, in CTA order, and writes its rows. One warp per row;
-// blockIdx.y spreads the rows.
-template <typename T, typename A>
-__global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constant__ PagedArgs a, int ctas) {
+// began and did not end, in CTA order, and writes its rows: a warp per row,
+// blockIdx.y spreads the rows. It is launched with the attention kernel still
+// running (programmatic dependent launch) and waits for it here: the launch and
+// the first instructions cost nothing then.
+constexpr int kCombineWarps = 8;
+template <typename T, typename A, int W>
+__global__ void __launch_bounds__(kCombineWarps * 32) paged_combine_kernel(const __grid_constant__ PagedArgs a,
+                                                                           int ctas) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int c = blockIdx.x;
-  const int b = a.meta[4 * c + 1];
+  const int4 meta = *reinterpret_cast<const int4*>(a.meta + 4 * c);
+  const int b = meta.y, h = meta.z, u = meta.w, D = a.D;
   if (b < 0) return;
-  const int h = a.meta[4 * c + 2], u = a.meta[4 * c + 3], D = a.D;
   int last = c + 1;
   while (last < ctas - 1 && a.meta[4 * last] == 0) ++last;
   const PagedReq req = paged_req(a, b);
   const long long row0 = static_cast<long long>(u) * a.unit_rows;
   const int rows = static_cast<int>(min(static_cast<long long>(a.unit_rows), static_cast<long long>(req.n) * a.G - row0));
   const long long size = static_cast<long long>(a.frag_rows) * (D + 1);
-  const A* frag = static_cast<const A*>(a.frag);
+  const A* first = static_cast<const A*>(a.frag) + (2LL * c + 1) * size;
+  const A* rest = static_cast<const A*>(a.frag) + 2LL * (c + 1) * size;  // of CTA c + 1; 2 * size apart
+  const int nrest = last - c;
   const A sink = sizeof(A) == 8 ? static_cast<A>(a.sink_d) : static_cast<A>(a.sink);
   const int lane = threadIdx.x & 31;
-  for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.y * 8) {
-    A den = frag[(2LL * c + 1) * size + static_cast<long long>(a.frag_rows) * D + r];
-    for (int x = c + 1; x <= last; ++x) den += frag[2LL * x * size + static_cast<long long>(a.frag_rows) * D + r];
+  const long long den_at = static_cast<long long>(a.frag_rows) * D;
+  for (int r = blockIdx.y * kCombineWarps + (threadIdx.x >> 5); r < rows; r += gridDim.y * kCombineWarps) {
+    A den = first[den_at + r];
+#pragma unroll 4
+    for (int x = 0; x < nrest; ++x) den += rest[2LL * x * size + den_at + r];
     den += sink;
-    const long long row = row0 + r, tok = req.tok0 + row / a.G;
-    const long long orow = tok * a.Hkv * a.G + static_cast<long long>(h) * a.G + row % a.G;
-    for (int col = lane; col < D; col += 32) {
+    const long long row = row0 + r, tok = row / a.G;
+    const long long orow = (req.tok0 + tok) * a.Hkv * a.G + static_cast<long long>(h) * a.G + (row - tok * a.G);
+    T* out = static_cast<T*>(a.out) + orow * D;
+    for (int col = lane * W; col < D; col += 32 * W) {
       const long long at = static_cast<long long>(r) * D + col;
-      A sum = frag[(2LL * c + 1) * size + at];
-      for (int x = c + 1; x <= last; ++x) sum += frag[2LL * x * size + at];
-      static_cast<T*>(a.out)[orow * D + col] = from_acc<T>(den > A(0) ? sum / den : A(0));
+      A sum[W];
+      auto add = [&](const A* f, bool set) {
+        alignas(16) A v[W];
+        if constexpr (W * sizeof(A) == 16)
+          *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(f + at);
+        else
+          v[0] = f[at];
+#pragma unroll
+        for (int i = 0; i < W; ++i) sum[i] = set ? v[i] : sum[i] + v[i];
+      };
+      add(first, true);
+#pragma unroll 4
+      for (int x = 0; x < nrest; ++x) add(rest + 2LL * x * size, false);
+      alignas(16) T y[W];
+#pragma unroll
+      for (int i = 0; i < W; ++i) y[i] = from_acc<T>(den > A(0) ? sum[i] / den : A(0));
+      if constexpr (W * sizeof(T) == 8) {
+        *reinterpret_cast<uint2*>(out + col) = *reinterpret_cast<const uint2*>(y);
+      } else if constexpr (W * sizeof(T) == 16) {
+        *reinterpret_cast<uint4*>(out + col) = *reinterpret_cast<const uint4*>(y);
+      } else {
+        out[col] = y[0];
+      }
     }
     if (lane == 0 && a.dtot) static_cast<A*>(a.dtot)[orow] = den;
   }
@@ -259,12 +290,31 @@ cudaError_t launch_simt_type(const PagedArgs& a, int ctas, cudaStream_t stream) 
   }
 }
 
+template <typename T, typename A, int W>
+cudaError_t launch_combine_w(const PagedArgs& a, int ctas, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg{};
+  int y = (a.frag_rows + kCombineWarps - 1) / kCombineWarps;
+  if (y > 8) y = 8;  // 147 x 8 CTAs fill the SMs once
+  cfg.gridDim = dim3(ctas - 1, y);
+  cfg.blockDim = dim3(kCombineWarps * 32);
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, paged_combine_kernel<T, A, W>, a, ctas);
+}
+
+// 16 bytes of sums per lane where rows start on 16 bytes in the fragments and
+// on a lane's share of 16 bytes in `out`.
 template <typename T, typename A>
 cudaError_t launch_combine(const PagedArgs& a, int ctas, cudaStream_t stream) {
   if (ctas < 2) return cudaSuccess;
-  const dim3 grid(ctas - 1, (a.frag_rows + 63) / 64);
-  paged_combine_kernel<T, A><<<grid, 256, 0, stream>>>(a, ctas);
-  return cudaGetLastError();
+  constexpr int W = 16 / sizeof(A);
+  if (a.D % W == 0 && reinterpret_cast<uintptr_t>(a.out) % (W * sizeof(T)) == 0)
+    return launch_combine_w<T, A, W>(a, ctas, stream);
+  return launch_combine_w<T, A, 1>(a, ctas, stream);
 }
 
 int sm_count() {

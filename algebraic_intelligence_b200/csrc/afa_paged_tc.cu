@@ -188,6 +188,7 @@ __global__ void __launch_bounds__(576, 1)
     tmem_relinquish();
   }
   tc_fence_before();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // see paged_combine_kernel
   PagedWalk walk;
   walk.init(a, paged_share<C::kThreads>(a, reinterpret_cast<long long*>(smem + C::SHARE_OFF)));
   __syncthreads();
@@ -217,13 +218,15 @@ __global__ void __launch_bounds__(576, 1)
                         p.r.tok0 + (p.u * 2 + i) * tile_tok);
       }
       ++qn;
-      auto load = [&](int i, bool v) {  // tile i of the piece
+      // This lane's page of tile i; outside the cache (zeros) where there is none.
+      auto page_of = [&](int i) {
         const int key = (p.t0 + i) * kPagedTile + lane * box_rows;
-        int page = a.num_pages;  // outside the cache: zeros
-        if (lane < per_tile && key < p.r.len) {
-          const int e = a.table[p.b * a.table_ld + (key >> a.page_shift)];
-          page = e >= 0 && e < a.num_pages ? e : a.num_pages;
-        }
+        if (i >= g.n || lane >= per_tile || key >= p.r.len) return a.num_pages;
+        const int e = a.table[p.b * a.table_ld + (key >> a.page_shift)];
+        return e >= 0 && e < a.num_pages ? e : a.num_pages;
+      };
+      auto load = [&](int i, bool v, int page) {  // tile i of the piece
+        const int key = (p.t0 + i) * kPagedTile + lane * box_rows;
         const int slot = u % C::NSLOT;
         if (!(ok = ok && __all_sync(0xffffffffu, mbar_wait(kv_empty + slot, ((u / C::NSLOT) & 1) ^ 1, a.status,
                                                            kDevTimeoutProducer))))
@@ -236,11 +239,24 @@ __global__ void __launch_bounds__(576, 1)
                         v ? &tm_v : &tm_k, kv_full + slot, 64 * h, key & (ps - 1), p.h, page);
         ++u;
       };
-      const int ahead = g.split ? 2 : 1;
-      for (int i = 0; ok && i < min(ahead, g.n); ++i) load(i, false);
+      // Table entries are read three tiles ahead of their loads' use, so no
+      // load waits for them.
+      int page[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) page[i] = page_of(i);
+      load(0, false, page[0]);
+      if (g.split && g.n > 1) load(1, false, page[1]);
       for (int i = 0; ok && i < g.n; ++i) {
-        load(i, true);
-        if (ok && i + ahead < g.n) load(i + ahead, false);
+        load(i, true, page[0]);
+        if (g.split) {
+          if (ok && i + 2 < g.n) load(i + 2, false, page[2]);
+        } else {
+          if (ok && i + 1 < g.n) load(i + 1, false, page[1]);
+        }
+        page[0] = page[1];
+        page[1] = page[2];
+        page[2] = page[3];
+        page[3] = page_of(i + 4);
       }
     }
     // Do not leave the CTA while loads into its shared memory are in flight.
