@@ -430,12 +430,13 @@ extern "C" int afa_paged(const void* q, const long long* q_strides, const void* 
   if (ctas > kMaxPagedCtas) ctas = kMaxPagedCtas;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool tc = paged_tc_supported(a, dtype);
-  a.unit_rows = tc ? paged_tc_unit_rows(a.G) : kSimtRows;
+  const int nt = tc ? paged_tr_rows(batch, tokens, a.G) : 0;
+  a.unit_rows = nt ? nt / a.G * a.G : tc ? paged_tc_unit_rows(a.G) : kSimtRows;
   a.frag_rows = frag_rows_of(a.unit_rows, tokens, a.G);
   const char* detail = "";
   cudaError_t e;
   if (tc) {
-    e = launch_paged_tc(a, ctas, st, &detail);
+    e = nt ? launch_paged_tr(a, nt, ctas, st, &detail) : launch_paged_tc(a, ctas, st, &detail);
   } else switch (dtype) {
     case kF64: e = launch_simt_type<double, double>(a, ctas, st); break;
     case kF32: e = launch_simt_type<float, float>(a, ctas, st); break;

@@ -34,8 +34,8 @@
 #include "afa_common.cuh"
 #include "afa_internal.h"
 #include "afa_paged.cuh"
+#include "afa_paged_tma.cuh"
 #include "afa_tc_shared.cuh"
-#include "afa_tmap.h"
 
 namespace afa {
 namespace {
@@ -67,14 +67,6 @@ struct PgCfg {
     return static_cast<uint32_t>((kk >> 1) * 32 + (kk & 1) * 8);
   }
 };
-
-__device__ __forceinline__ void tma_load_4d(void* dst, const void* tmap, uint64_t* bar, int c0, int c1, int c2, int c3) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
-      "l"(tmap), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
-      : "memory");
-}
 
 // Octic map of one 32-column chunk of a score row into 16 packed bf16 pairs;
 // returns the fp32 sum of the weights. MASK: bit e of `seen` tells whether the
@@ -198,9 +190,7 @@ __global__ void __launch_bounds__(576, 1)
 
   if (warp == C::kTmaWarp) {
     // ------------------------------------------------------------------ TMA
-    const int ps = 1 << a.page_shift;
-    const int per_tile = ps < kPagedTile ? kPagedTile >> a.page_shift : 1;
-    const int box_rows = ps < kPagedTile ? ps : kPagedTile;
+    KvPages pages(a);
     int u = 0, qn = 0;
     bool ok = true;
     while (ok && walk.next(a, p)) {
@@ -218,32 +208,22 @@ __global__ void __launch_bounds__(576, 1)
                         p.r.tok0 + (p.u * 2 + i) * tile_tok);
       }
       ++qn;
-      // This lane's page of tile i; outside the cache (zeros) where there is none.
-      auto page_of = [&](int i) {
-        const int key = (p.t0 + i) * kPagedTile + lane * box_rows;
-        if (i >= g.n || lane >= per_tile || key >= p.r.len) return a.num_pages;
-        const int e = a.table[p.b * a.table_ld + (key >> a.page_shift)];
-        return e >= 0 && e < a.num_pages ? e : a.num_pages;
-      };
       auto load = [&](int i, bool v, int page) {  // tile i of the piece
-        const int key = (p.t0 + i) * kPagedTile + lane * box_rows;
         const int slot = u % C::NSLOT;
         if (!(ok = ok && __all_sync(0xffffffffu, mbar_wait(kv_empty + slot, ((u / C::NSLOT) & 1) ^ 1, a.status,
                                                            kDevTimeoutProducer))))
           return;
         if (lane == 0) mbar_arrive_expect_tx(kv_full + slot, C::TILE_BYTES);
         __syncwarp();
-        if (lane < per_tile)
-          for (int h = 0; h < C::KSUB; ++h)
-            tma_load_4d(smem + C::KV_OFF + (slot * C::KSUB + h) * C::SUB_BYTES + lane * box_rows * 128,
-                        v ? &tm_v : &tm_k, kv_full + slot, 64 * h, key & (ps - 1), p.h, page);
+        pages.template load<C::KSUB>(smem + C::KV_OFF + slot * C::TILE_BYTES, v ? &tm_v : &tm_k, kv_full + slot,
+                                     p, i, page);
         ++u;
       };
       // Table entries are read three tiles ahead of their loads' use, so no
       // load waits for them.
       int page[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) page[i] = page_of(i);
+      for (int i = 0; i < 4; ++i) page[i] = pages.page(a, p, i);
       load(0, false, page[0]);
       if (g.split && g.n > 1) load(1, false, page[1]);
       for (int i = 0; ok && i < g.n; ++i) {
@@ -256,7 +236,7 @@ __global__ void __launch_bounds__(576, 1)
         page[0] = page[1];
         page[1] = page[2];
         page[2] = page[3];
-        page[3] = page_of(i + 4);
+        page[3] = pages.page(a, p, i + 4);
       }
     }
     // Do not leave the CTA while loads into its shared memory are in flight.
@@ -296,19 +276,9 @@ __global__ void __launch_bounds__(576, 1)
       const PgPiece g = pg_piece(a, p, tile_rows);
       const int n = g.n;
       if (n == 0) continue;
-      // V of tile i: rows behind the request's last token, up to their page's end.
       auto clear_tail = [&](int i, int slot) {
-        const int lim = p.r.len - (p.t0 + i) * kPagedTile;
-        if (lim >= kPagedTile) return;
-        const int ps = 1 << a.page_shift;
-        const int end = min(kPagedTile, (lim + ps - 1) & ~(ps - 1));
-        uint8_t* base = smem + C::KV_OFF + slot * C::TILE_BYTES;
-        for (int x = lim * 8 + lane; x < end * 8; x += 32)
-#pragma unroll
-          for (int h = 0; h < C::KSUB; ++h)
-            st_shared_v4(smem_u32(base + h * C::SUB_BYTES + x * 16), make_uint4(0u, 0u, 0u, 0u));
-        fence_proxy_async_shared();
-        __syncwarp();
+        clear_v_tail<C::KSUB>(smem + C::KV_OFF + slot * C::TILE_BYTES, p.r.len - (p.t0 + i) * kPagedTile, a.page_shift,
+                              lane);
       };
       if (!(ok = __all_sync(0xffffffffu, mbar_wait(q_full, qn & 1, a.status, kDevTimeoutMma)))) break;
       ++qn;
@@ -589,24 +559,6 @@ __global__ void __launch_bounds__(576, 1)
   }
 }
 
-// A bf16 tensor map of four dimensions, box 64 x b1 x 1 x b3 (or 64 x b1 x b2 x
-// 1), 128-byte swizzle; strides in elements, from the second dimension on.
-bool map_4d(CUtensorMap* m, const void* base, const long long (&dims)[4], const long long (&strides)[3],
-            const int (&box)[4]) {
-  auto fn = encode_fn();
-  if (!fn) return false;
-  cuuint64_t d[4], s[3];
-  cuuint32_t b[4], e[4] = {1, 1, 1, 1};
-  for (int i = 0; i < 4; ++i) {
-    d[i] = static_cast<cuuint64_t>(dims[i]);
-    b[i] = static_cast<cuuint32_t>(box[i]);
-  }
-  for (int i = 0; i < 3; ++i) s[i] = static_cast<cuuint64_t>(strides[i]) * 2;
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), d, s, b, e,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int HD>
 cudaError_t launch_hd(const PagedArgs& a, int ctas, cudaStream_t stream, const char** detail) {
   using C = PgCfg<HD>;
@@ -621,11 +573,8 @@ cudaError_t launch_hd(const PagedArgs& a, int ctas, cudaStream_t stream, const c
     *detail = "kernel set-up failed (max dynamic shared memory attribute)";
     return e;
   }
-  const int ps = 1 << a.page_shift, rows = ps < kPagedTile ? ps : kPagedTile;
   CUtensorMap tq, tk, tv;
-  if (!map_4d(&tq, a.q, {HD, a.G, a.Hkv, a.T}, {a.q_sh, a.q_sh * a.G, a.q_st}, {64, a.G, 1, 128 / a.G}) ||
-      !map_4d(&tk, a.k, {HD, ps, a.Hkv, a.num_pages}, {a.k_sr, a.k_sh, a.k_sp}, {64, rows, 1, 1}) ||
-      !map_4d(&tv, a.v, {HD, ps, a.Hkv, a.num_pages}, {a.v_sr, a.v_sh, a.v_sp}, {64, rows, 1, 1})) {
+  if (!paged_tmaps(a, 128 / a.G, &tq, &tk, &tv)) {
     *detail = "cuTensorMapEncodeTiled failed";
     return cudaErrorInvalidValue;
   }

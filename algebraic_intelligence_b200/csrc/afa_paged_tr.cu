@@ -1,0 +1,480 @@
+// AFA over a paged cache for few query rows per key head (single tokens, small
+// trees), bf16, head_dim 64 or 128, on the tensor cores with the scores
+// transposed. Math and work split: afa_paged.cu, afa_paged.cuh.
+//
+//   S^T = K Q^T     M = 128 keys, N = NT query rows
+//   O^T += V^T P^T  M = head_dim,  N = NT, over the tile's 128 keys
+//
+// The query rows are the narrow side of both products, so the tensor core and
+// the octic map work on NT (16, 32 or 64) rows and not on the 128 that a row
+// tile of the other kernel has: a thread owns one key and maps NT scores, and
+// every warp has the same share whatever the number of rows. What is left is
+// the cache's bytes. With so little to map, each weight is computed in the form
+// that is exact in the negative tail (octic_exact2).
+//
+//   warp 8      TMA: K and V tiles through a ring, in the order they are used;
+//               Q double buffered, so the next unit's loads never wait.
+//   warp 9      every tcgen05.mma, and the clearing of V rows behind a request's
+//               last token (see afa_paged_tc.cu).
+//   warps 0-7   two groups of four warps take tiles in turn: scores from TMEM,
+//               P^T to shared memory as bf16 ([key][row], 128-byte swizzle: the
+//               layout V has), row sums in registers. One group maps while the
+//               tensor core works on the other's tile.
+// TMEM columns: S^T of group g at [NT g, NT g + NT), O^T at [128, 128 + NT).
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include "afa_common.cuh"
+#include "afa_internal.h"
+#include "afa_paged.cuh"
+#include "afa_paged_tma.cuh"
+
+namespace afa {
+namespace {
+
+template <int HD, int NT>
+struct TrCfg {
+  static constexpr int kMapWarps = 8;
+  static constexpr int kTmaWarp = 8;
+  static constexpr int kMmaWarp = 9;
+  static constexpr int kThreads = 10 * 32;
+  static constexpr int KSUB = HD / 64;
+  static constexpr int SUB_BYTES = 128 * 128;
+  static constexpr int TILE_BYTES = KSUB * SUB_BYTES;
+  static constexpr int QSUB_BYTES = NT * 128;
+  static constexpr int Q_BYTES = KSUB * QSUB_BYTES;
+  static constexpr int P_BYTES = 128 * 128;
+  static constexpr int Q_OFF = 0;
+  static constexpr int P_OFF = 2 * Q_BYTES;
+  static constexpr int KV_OFF = P_OFF + 2 * P_BYTES;
+  static constexpr int NSLOT = HD == 128 ? 5 : 8;
+  static constexpr int BAR_OFF = KV_OFF + NSLOT * TILE_BYTES;
+  static constexpr int NBAR = 4 + 2 * NSLOT + 2 + 2 + 1 + 1;
+  static constexpr int TMEM_OFF = BAR_OFF + NBAR * 8;
+  // fp32 row sums [warp][row], then the totals [row]: in group 0's P, which no
+  // product reads any more when they are written.
+  static constexpr int RED_OFF = P_OFF;
+  static constexpr int SHARE_OFF = TMEM_OFF + 16;
+  static_assert((kMapWarps + 1) * NT * 4 <= P_BYTES, "row sums fit in P");
+  static constexpr int SMEM_BYTES = SHARE_OFF + (kThreads / 32 + 4) * 8 + 1024;
+  static_assert(Q_BYTES % 1024 == 0 && SMEM_BYTES <= 227 * 1024, "shared memory per CTA");
+  static constexpr uint32_t TMEM_COLS = 256;
+  static constexpr uint32_t O_COL = 128;
+};
+
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+}
+
+// Sums of 16 values over the warp's lanes: lane l returns value l / 2's.
+__device__ __forceinline__ float reduce16(float (&v)[16], int lane) {
+#pragma unroll
+  for (int m = 8; m >= 1; m >>= 1) {
+    const bool hi = (lane & (2 * m)) != 0;
+#pragma unroll
+    for (int i = 0; i < m; ++i) {
+      const float send = hi ? v[i] : v[i + m];
+      const float keep = hi ? v[i + m] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, 2 * m);
+    }
+  }
+  return v[0] + __shfl_xor_sync(0xffffffffu, v[0], 1);
+}
+
+template <int HD, int NT>
+__global__ void __launch_bounds__(320, 1)
+    afa_paged_tr_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                        const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PagedArgs a) {
+  using C = TrCfg<HD, NT>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
+  uint64_t* q_full = bars;
+  uint64_t* q_empty = bars + 2;
+  uint64_t* kv_full = bars + 4;
+  uint64_t* kv_empty = kv_full + C::NSLOT;
+  uint64_t* s_full = kv_empty + C::NSLOT;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_full = p_full + 2;
+  uint64_t* drain = o_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::TMEM_OFF);
+  float* red = reinterpret_cast<float*>(smem + C::RED_OFF);
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(q_full + i, 1);
+      mbar_init(q_empty + i, 1);
+      mbar_init(s_full + i, 1);
+      mbar_init(p_full + i, 4);  // one elected arrive per warp of the group
+    }
+    for (int s = 0; s < C::NSLOT; ++s) {
+      mbar_init(kv_full + s, 1);
+      mbar_init(kv_empty + s, 1);
+    }
+    mbar_init(o_full, 1);
+    mbar_init(drain, 1);
+    fence_barrier_init();
+    fence_proxy_async_smem();
+    prefetch_tmap(&tm_q);
+    prefetch_tmap(&tm_k);
+    prefetch_tmap(&tm_v);
+    paged_meta_clear(a.meta);
+  }
+  if (warp == C::kMmaWarp) {
+    tmem_alloc(tmem_slot, C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // see paged_combine_kernel
+  PagedWalk walk;
+  walk.init(a, paged_share<C::kThreads>(a, reinterpret_cast<long long*>(smem + C::SHARE_OFF)));
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  PagedPiece p;
+
+  if (warp == C::kTmaWarp) {
+    // ------------------------------------------------------------------ TMA
+    KvPages pages(a);
+    int u = 0, qn = 0;
+    bool ok = true;
+    while (ok && walk.next(a, p)) {
+      if (lane == 0) paged_meta_piece(a.meta, p);
+      const int n = p.tiles > 0 ? p.t1 - p.t0 : 0;
+      if (n == 0) continue;
+      const int qb = qn & 1;
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(q_empty + qb, ((qn >> 1) & 1) ^ 1, a.status, kDevTimeoutProducer))))
+        break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(q_full + qb, C::KSUB * a.unit_rows * 128);
+        for (int h = 0; h < C::KSUB; ++h)
+          tma_load_4d(smem + C::Q_OFF + qb * C::Q_BYTES + h * C::QSUB_BYTES, &tm_q, q_full + qb, 64 * h, 0, p.h,
+                      p.r.tok0 + p.u * (a.unit_rows / a.G));
+      }
+      ++qn;
+      auto load = [&](int i, bool v, int page) {
+        const int slot = u % C::NSLOT;
+        if (!(ok = ok && __all_sync(0xffffffffu, mbar_wait(kv_empty + slot, ((u / C::NSLOT) & 1) ^ 1, a.status,
+                                                           kDevTimeoutProducer))))
+          return;
+        if (lane == 0) mbar_arrive_expect_tx(kv_full + slot, C::TILE_BYTES);
+        __syncwarp();
+        pages.template load<C::KSUB>(smem + C::KV_OFF + slot * C::TILE_BYTES, v ? &tm_v : &tm_k, kv_full + slot,
+                                     p, i, page);
+        ++u;
+      };
+      int page[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) page[i] = pages.page(a, p, i);
+      load(0, false, page[0]);
+      if (n > 1) load(1, false, page[1]);
+      for (int i = 0; ok && i < n; ++i) {
+        load(i, true, page[0]);
+        if (ok && i + 2 < n) load(i + 2, false, page[2]);
+        page[0] = page[1];
+        page[1] = page[2];
+        page[2] = page[3];
+        page[3] = pages.page(a, p, i + 4);
+      }
+    }
+    // Do not leave the CTA while loads into its shared memory are in flight.
+    for (int x = qn - 2 < 0 ? 0 : qn - 2; x < qn; ++x) (void)mbar_wait(q_full + (x & 1), (x >> 1) & 1, nullptr, 0);
+    for (int x = u - C::NSLOT < 0 ? 0 : u - C::NSLOT; x < u; ++x)
+      (void)mbar_wait(kv_full + (x % C::NSLOT), (x / C::NSLOT) & 1, nullptr, 0);
+  } else if (warp == C::kMmaWarp) {
+    // ------------------------------------------------------------------ MMA
+    constexpr uint32_t idesc_s = idesc_bf16_f32(128, NT, false);
+    constexpr uint32_t idesc_o = idesc_bf16_f32(HD, NT, true) | (1u << 15);  // A = V^T: its M (head_dim) is contiguous
+    const uint64_t q_desc = sw128_desc(smem_u32(smem + C::Q_OFF), 16, 1024);
+    const uint64_t k_desc = sw128_desc(smem_u32(smem + C::KV_OFF), 16, 1024);
+    const uint64_t v_desc = sw128_desc(smem_u32(smem + C::KV_OFF), C::SUB_BYTES, 1024);
+    const uint64_t p_desc = sw128_desc(smem_u32(smem + C::P_OFF), C::SUB_BYTES, 1024);
+    auto issue_s = [&](int g, int qb, int slot) {
+      const uint64_t kb = desc_add(k_desc, slot * C::TILE_BYTES), qd = desc_add(q_desc, qb * C::Q_BYTES);
+#pragma unroll
+      for (int kk = 0; kk < HD / 16; ++kk)
+        umma_ss(tmem + g * NT, desc_add(kb, (kk >> 2) * C::SUB_BYTES + (kk & 3) * 32),
+                desc_add(qd, (kk >> 2) * C::QSUB_BYTES + (kk & 3) * 32), idesc_s, kk > 0 ? 1u : 0u);
+    };
+    auto issue_o = [&](int g, int slot, bool acc) {
+      const uint64_t vb = desc_add(v_desc, slot * C::TILE_BYTES), pd = desc_add(p_desc, g * C::P_BYTES);
+#pragma unroll
+      for (int kk = 0; kk < kPagedTile / 16; ++kk)
+        umma_ss(tmem + C::O_COL, desc_add(vb, kk * 2048), desc_add(pd, kk * 2048), idesc_o, (acc || kk > 0) ? 1u : 0u);
+    };
+    int qn = 0, u = 0, pc0 = 0, pc1 = 0;
+    bool ok = true;
+    auto wait_kv = [&](int x) {
+      return __all_sync(0xffffffffu,
+                        mbar_wait(kv_full + x % C::NSLOT, (x / C::NSLOT) & 1, a.status, kDevTimeoutMma));
+    };
+    while (ok && walk.next(a, p)) {
+      const int n = p.tiles > 0 ? p.t1 - p.t0 : 0;
+      if (n == 0) continue;
+      const int qb = qn & 1;
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(q_full + qb, (qn >> 1) & 1, a.status, kDevTimeoutMma)))) break;
+      ++qn;
+      for (int i = 0; ok && i < min(2, n); ++i, ++u) {
+        if (!(ok = wait_kv(u))) break;
+        tc_fence_after();
+        if (lane == 0) {
+          issue_s(i, qb, u % C::NSLOT);
+          umma_commit(s_full + i);
+          umma_commit(kv_empty + u % C::NSLOT);
+          if (i + 1 == n) umma_commit(q_empty + qb);
+        }
+      }
+      for (int i = 0; ok && i < n; ++i) {
+        const int g = i & 1, sv = u % C::NSLOT, sk = (u + 1) % C::NSLOT;
+        const bool more = i + 2 < n;
+        if (!(ok = wait_kv(u))) break;
+        clear_v_tail<C::KSUB>(smem + C::KV_OFF + sv * C::TILE_BYTES, p.r.len - (p.t0 + i) * kPagedTile, a.page_shift,
+                              lane);
+        if (more && !(ok = wait_kv(u + 1))) break;
+        const int phase = g ? pc1++ : pc0++;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(p_full + g, phase & 1, a.status, kDevTimeoutMma)))) break;
+        tc_fence_after();
+        if (lane == 0) {
+          issue_o(g, sv, i > 0);
+          umma_commit(kv_empty + sv);
+          if (i + 1 == n) umma_commit(o_full);
+          if (more) {
+            issue_s(g, qb, sk);
+            umma_commit(s_full + g);
+            umma_commit(kv_empty + sk);
+            if (i + 3 == n) umma_commit(q_empty + qb);
+          }
+        }
+        u += more ? 2 : 1;
+      }
+    }
+    // Every MMA issued must finish before TMEM is released.
+    if (lane == 0) {
+      umma_commit(drain);
+      (void)mbar_wait(drain, 0, nullptr, 0);
+    }
+    __syncwarp();
+  } else {
+    // --------------------------------------------------- octic map + epilogue
+    const int g = warp >> 2;    // group: tiles g, g + 2, ... of a piece
+    const int sub = warp & 3;   // TMEM lane quarter
+    const uint32_t lane_off = static_cast<uint32_t>(sub * 32) << 16;
+    const float2 sc = make_float2(a.scale, a.scale);
+    const int krow = sub * 32 + lane;  // this thread's key of a tile
+    const uint32_t p_row = smem_u32(smem + C::P_OFF + g * C::P_BYTES + krow * 128);
+    int scnt = 0, oc = 0;
+    bool ok = true;
+    auto sync_map = [] { asm volatile("bar.sync 1, %0;" ::"r"(C::kMapWarps * 32) : "memory"); };
+    // Every warp walks every piece and meets at the same barriers, also after
+    // a wait ran out (ok false).
+    while (walk.next(a, p)) {
+      const int n = p.tiles > 0 ? p.t1 - p.t0 : 0;
+      const long long row0 = static_cast<long long>(p.u) * a.unit_rows;
+      const long long left = static_cast<long long>(p.r.n) * a.G - row0;
+      const int rows = left < a.unit_rows ? static_cast<int>(left) : a.unit_rows;
+      const int tok_u = p.u * (a.unit_rows / a.G);  // first new token of the unit
+      const int prefix = p.r.len - p.r.n;
+      float sum[NT];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) sum[i] = 0.f;
+      for (int i = g; i < n && ok; i += 2) {
+        const int key = (p.t0 + i) * kPagedTile + krow;
+        bool in = key < p.r.len;
+        if (in) {
+          const int e = a.table[p.b * a.table_ld + (key >> a.page_shift)];
+          in = e >= 0 && e < a.num_pages;
+        }
+        // Rows that see this thread's key.
+        unsigned long long seen = in ? ~0ull : 0ull;
+        const int at = key - prefix;
+        if (in && at >= 0) {
+          if (a.anc) {
+            seen = 0;
+            const int w = at >> 5;
+            if (w < a.words)
+              for (int j = 0; j * a.G < rows; ++j) {
+                const unsigned word = a.anc[static_cast<long long>(p.r.tok0 + tok_u + j) * a.anc_ld + w];
+                if ((word >> (at & 31)) & 1u) seen |= ((1ull << (a.G - 1)) * 2 - 1) << (j * a.G);
+              }
+          } else {
+            const long long first = static_cast<long long>(at) * a.G - row0;  // first row of token `at`
+            seen = first <= 0 ? ~0ull : first >= 64 ? 0ull : ~0ull << first;
+          }
+        }
+        ok = __all_sync(0xffffffffu, mbar_wait(s_full + g, scnt & 1, a.status, kDevTimeoutSoftmax));
+        ++scnt;
+        if (!ok) break;
+        tc_fence_after();
+        __syncwarp();
+        constexpr int W = NT < 32 ? NT : 32;  // columns per TMEM load
+#pragma unroll
+        for (int c0 = 0; c0 < NT; c0 += W) {
+          uint32_t sv[W];
+          if constexpr (W == 32)
+            tmem_ld32(tmem + g * NT + lane_off + c0, sv);
+          else
+            tmem_ld16(tmem + g * NT + lane_off + c0, sv);
+          tmem_ld_wait();
+          const unsigned word = static_cast<unsigned>(seen >> c0);
+#pragma unroll
+          for (int c = 0; c < W; c += 8) {
+            uint32_t pk[4];
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+              const float2 s = __fmul2_rn(make_float2(__uint_as_float(sv[c + e]), __uint_as_float(sv[c + e + 1])), sc);
+              float2 w = octic_exact2(s);
+              w.x = (word >> (c + e)) & 1u ? w.x : 0.f;
+              w.y = (word >> (c + e + 1)) & 1u ? w.y : 0.f;
+              sum[c0 + c + e] += w.x;
+              sum[c0 + c + e + 1] += w.y;
+              pk[e >> 1] = pack_bf16x2(w.x, w.y);
+            }
+            // 16-byte chunk j of key row k lies at (j ^ (k % 8)) * 16.
+            const int j = (c0 + c) >> 3;
+            st_shared_v4(p_row + ((j ^ (krow & 7)) << 4), make_uint4(pk[0], pk[1], pk[2], pk[3]));
+          }
+        }
+        fence_proxy_async_shared();  // P is read by the tensor core
+        tc_fence_before();           // and the scores may be overwritten
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + g);
+      }
+      if (n > 0) {
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(o_full, oc & 1, a.status, kDevTimeoutEpilogue));
+        ++oc;
+      }
+      // Row sums over the lanes, then over the eight warps in a fixed order.
+#pragma unroll
+      for (int c = 0; c < NT; c += 16) {
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = sum[c + i];
+        const float s = reduce16(v, lane);
+        if ((lane & 1) == 0) red[warp * NT + c + (lane >> 1)] = s;
+      }
+      sync_map();
+      if (threadIdx.x < NT) {
+        float t = 0.f;
+#pragma unroll
+        for (int w = 0; w < C::kMapWarps; ++w) t += red[w * NT + threadIdx.x];
+        red[C::kMapWarps * NT + threadIdx.x] = t;
+      }
+      sync_map();
+      tc_fence_after();
+      const bool whole = p.whole(), o_here = ok && n > 0;
+      // Head channel of this thread's TMEM lane: with 64 channels (M = 64) the
+      // accumulator uses 16 lanes of every quarter.
+      const bool chan = HD == 128 || lane < 16;
+      const int d = HD == 128 ? krow : sub * 16 + (lane & 15);
+      const float* tot = red + C::kMapWarps * NT;
+      float* frag = static_cast<float*>(a.frag) + (2LL * blockIdx.x + paged_frag_slot(p)) * a.frag_rows * (HD + 1);
+      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out);
+      // The groups share the rows: 8 at a time, alternately.
+      int tok = tok_u, head = 0;  // of row c, kept up without a division
+#pragma unroll 1
+      for (int c = 0; c < NT && c < rows; c += 8) {
+        if (((c >> 3) & 1) == g) {
+          uint32_t ov[8];
+          __syncwarp();
+          if (o_here) {
+            tmem_ld8(tmem + C::O_COL + lane_off + c, ov);
+            tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ov[e] = 0u;
+          }
+          int t = tok, hh = head;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            if (c + e < rows) {
+              const float den = tot[c + e] + a.sink;
+              const long long orow = (static_cast<long long>(p.r.tok0) + t) * a.Hkv * a.G +
+                                     static_cast<long long>(p.h) * a.G + hh;
+              if (whole) {
+                const float y = den > 0.f ? __uint_as_float(ov[e]) / den : 0.f;
+                if (chan) out[orow * HD + d] = __float2bfloat16_rn(y);
+                if (a.dtot && threadIdx.x % 128 == 0) static_cast<float*>(a.dtot)[orow] = den;
+              } else {
+                if (chan) frag[static_cast<long long>(c + e) * HD + d] = __uint_as_float(ov[e]);
+                if (threadIdx.x % 128 == 0) frag[static_cast<long long>(a.frag_rows) * HD + c + e] = tot[c + e];
+              }
+            }
+            if (++hh == a.G) {
+              hh = 0;
+              ++t;
+            }
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (++head == a.G) {
+            head = 0;
+            ++tok;
+          }
+      }
+      // O and the sums are read: the next piece's first P may be announced.
+      tc_fence_before();
+      sync_map();
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == C::kMmaWarp) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, C::TMEM_COLS);
+  }
+}
+
+template <int HD, int NT>
+cudaError_t launch_nt(const PagedArgs& a, int ctas, cudaStream_t stream, const char** detail) {
+  using C = TrCfg<HD, NT>;
+  static PerDeviceOnce setup;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess)
+    e = setup.run(dev, [&] {
+      return cudaFuncSetAttribute(afa_paged_tr_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  C::SMEM_BYTES);
+    });
+  if (e != cudaSuccess) {
+    *detail = "kernel set-up failed (max dynamic shared memory attribute)";
+    return e;
+  }
+  CUtensorMap tq, tk, tv;
+  if (!paged_tmaps(a, a.unit_rows / a.G, &tq, &tk, &tv)) {
+    *detail = "cuTensorMapEncodeTiled failed";
+    return cudaErrorInvalidValue;
+  }
+  afa_paged_tr_kernel<HD, NT><<<ctas, C::kThreads, C::SMEM_BYTES, stream>>>(tq, tk, tv, a);
+  return cudaGetLastError();
+}
+
+template <int HD>
+cudaError_t launch_hd(const PagedArgs& a, int nt, int ctas, cudaStream_t stream, const char** detail) {
+  switch (nt) {
+    case 16: return launch_nt<HD, 16>(a, ctas, stream, detail);
+    case 32: return launch_nt<HD, 32>(a, ctas, stream, detail);
+    default: return launch_nt<HD, 64>(a, ctas, stream, detail);
+  }
+}
+
+}  // namespace
+
+int paged_tr_rows(int B, int T, int G) {
+  const long long rows = (static_cast<long long>(T) + B - 1) / B * G;
+  for (int nt : {16, 32, 64})
+    if (rows <= nt) return nt;
+  return 0;
+}
+
+cudaError_t launch_paged_tr(const PagedArgs& a, int nt, int ctas, cudaStream_t stream, const char** detail) {
+  return a.D == 128 ? launch_hd<128>(a, nt, ctas, stream, detail) : launch_hd<64>(a, nt, ctas, stream, detail);
+}
+
+}  // namespace afa
