@@ -7,6 +7,7 @@ raises, naming the file it looked for.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from pathlib import Path
 
@@ -121,7 +122,29 @@ def accum_dtype(dt: torch.dtype) -> torch.dtype:
 
 
 def stream_ptr(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # The raw handle of torch.cuda.current_stream(device), without the Stream
+    # object around it (4 us of host time per call).
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+@functools.lru_cache(maxsize=4096)
+def longs(*values: int) -> ctypes.Array:
+    """A C array of long long (strides), read only and kept by its values: making one costs about 1 us."""
+    return (ctypes.c_longlong * len(values))(*values)
+
+
+@functools.lru_cache(maxsize=1024)
+def ints(*values: int) -> ctypes.Array:
+    """A C array of int, read only and kept by its values."""
+    return (ctypes.c_int * len(values))(*values)
+
+
+def call(device: torch.device, entry, *args) -> int:
+    """entry(*args, current stream) with `device` current."""
+    if torch.cuda.current_device() == device.index:
+        return entry(*args, stream_ptr(device))
+    with torch.cuda.device(device):
+        return entry(*args, stream_ptr(device))
 
 
 def device_status(device: torch.device, clear: bool = True) -> int:

@@ -49,6 +49,7 @@ class CayleyRotary(NamedTuple):
 
 
 _TORCH_DTYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float64": torch.float64}
+_TABLE_DTYPES = frozenset(_TORCH_DTYPES.values())
 
 
 def _torch_dtype(dtype) -> torch.dtype:
@@ -177,62 +178,67 @@ def axis_arguments(rotary_params, positions, sections, dim, shape, device) -> Ax
     is given."""
     if positions is None or sections is None:
         raise ValueError("a rotation needs positions and sections")
-    sections = tuple(int(n) for n in sections)
+    sections = tuple(map(int, sections))
+    pairs = dim // 2
     if not 1 <= len(sections) <= 4:
         raise ValueError("between one and four position axes are supported")
-    if any(n < 0 for n in sections) or sum(sections) > dim // 2:
-        raise ValueError(f"sections must be nonnegative and sum to at most {dim // 2}, got {sections}")
+    if min(sections) < 0 or sum(sections) > pairs:
+        raise ValueError(f"sections must be nonnegative and sum to at most {pairs}, got {sections}")
     c, s = _extract_cs(rotary_params)
-    c, s = (torch.from_numpy(np.ascontiguousarray(x)) if isinstance(x, np.ndarray) else x for x in (c, s))
-    if not isinstance(c, torch.Tensor) or not isinstance(s, torch.Tensor) or c.dtype not in _TORCH_DTYPES.values() \
+    if isinstance(c, np.ndarray):
+        c = torch.from_numpy(np.ascontiguousarray(c))
+    if isinstance(s, np.ndarray):
+        s = torch.from_numpy(np.ascontiguousarray(s))
+    if not isinstance(c, torch.Tensor) or not isinstance(s, torch.Tensor) or c.dtype not in _TABLE_DTYPES \
             or s.dtype != c.dtype:
         raise TypeError("the rotary tables must share a dtype: float32, bfloat16 or float64")
-    if c.shape != s.shape or c.ndim == 0 or c.shape[-1] != dim // 2 or c.numel() == 0:
-        raise ValueError(f"rotary tables must have shape (positions, {dim // 2}), got {tuple(c.shape)} and "
+    if c.shape != s.shape or c.ndim == 0 or c.shape[-1] != pairs or c.numel() == 0:
+        raise ValueError(f"rotary tables must have shape (positions, {pairs}), got {tuple(c.shape)} and "
                          f"{tuple(s.shape)}")
     if c.requires_grad or s.requires_grad:
         raise ValueError("the rotary tables have no gradient")
     p = positions if isinstance(positions, torch.Tensor) else torch.as_tensor(np.asarray(positions))
-    if p.dtype not in (torch.int32, torch.int64):
+    if p.dtype != torch.int32 and p.dtype != torch.int64:
         raise TypeError("positions must be int32 or int64")
-    if tuple(p.shape) != (len(sections), *shape):
+    if p.shape != (len(sections), *shape):
         raise ValueError(f"positions must have shape {(len(sections), *shape)}, got {tuple(p.shape)}")
-    length = c.numel() // (dim // 2)
+    length = c.numel() // pairs
     if not p.is_cuda and p.numel() and not (0 <= int(p.min()) and int(p.max()) < length):
         raise ValueError(f"positions must lie in [0, {length}), the tables' rows")
-    if device is not None:
+    if device is not None and not c.device == s.device == p.device == device:
         if any(x.is_cuda and x.device != device for x in (c, s, p)):
             raise ValueError(f"tables and positions must be on {device}")
         c, s, p = c.to(device), s.to(device), p.to(device)
-    c, s = (x.reshape(length, dim // 2).contiguous() for x in (c, s))
-    return AxisArguments(c, s, p, (ctypes.c_int * len(sections))(*sections))
+    if c.ndim != 2:
+        c, s = c.reshape(length, pairs), s.reshape(length, pairs)
+    return AxisArguments(c.contiguous(), s.contiguous(), p, _lib.ints(*sections))
+
+
+def _row_strides(t, token_major):
+    """Strides (batch, token, head) of the rows of t."""
+    return _lib.longs(0, *t.stride()[:2]) if token_major else _lib.longs(*(t.stride(i) for i in (0, 2, 1)))
 
 
 def _rotate_axes(q, k, axes: AxisArguments, backward: bool):
     """One launch: q and k (or None) turned, backward the other way; contiguous results."""
     token_major = q.ndim == 3
-    tensors = [t if t is None or t.stride(-1) == 1 else t.contiguous() for t in (q, k)]
-
-    def strides(t):  # batch, token, head
-        if t is None:
-            return None
-        return (ctypes.c_longlong * 3)(*((0, t.stride(0), t.stride(1)) if token_major else
-                                         (t.stride(0), t.stride(2), t.stride(1))))
-
-    outs = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in tensors]
+    q = q if q.stride(-1) == 1 else q.contiguous()
+    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ko = None
+    if k is not None:
+        k = k if k.stride(-1) == 1 else k.contiguous()
+        ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
     batch, tokens = (1, q.shape[0]) if token_major else (q.shape[0], q.shape[2])
-    p = axes.positions
-    p_strides = (p.stride(0), 0 if p.ndim == 2 else p.stride(1), p.stride(-1))
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    with torch.cuda.device(q.device):
-        rc = _lib.load().afa_ago_rotate_axes(
-            ptr(tensors[0]), strides(tensors[0]), ptr(outs[0]), q.shape[1], ptr(tensors[1]), strides(tensors[1]),
-            ptr(outs[1]), 0 if k is None else k.shape[1], axes.c.data_ptr(), axes.s.data_ptr(),
-            _lib.dtype_code(axes.c.dtype), axes.c.shape[0], p.data_ptr(), (ctypes.c_longlong * 3)(*p_strides),
-            int(p.dtype == torch.int64), axes.sections, p.shape[0], int(token_major), batch, tokens, q.shape[-1],
-            int(backward), _lib.dtype_code(q.dtype), _lib.stream_ptr(q.device))
+    c, p = axes.c, axes.positions
+    rc = _lib.call(
+        q.device, _lib.load().afa_ago_rotate_axes, q.data_ptr(), _row_strides(q, token_major), qo.data_ptr(),
+        q.shape[1], *((None, None, None, 0) if k is None else
+                      (k.data_ptr(), _row_strides(k, token_major), ko.data_ptr(), k.shape[1])),
+        c.data_ptr(), axes.s.data_ptr(), _lib.dtype_code(c.dtype), c.shape[0], p.data_ptr(),
+        _lib.longs(p.stride(0), 0 if p.ndim == 2 else p.stride(1), p.stride(-1)), p.dtype == torch.int64,
+        axes.sections, p.shape[0], token_major, batch, tokens, q.shape[-1], backward, _lib.dtype_code(q.dtype))
     _lib.check(rc, "afa_ago_rotate_axes")
-    return outs[0], outs[1]
+    return qo, ko
 
 
 class _RotateAxes(torch.autograd.Function):
@@ -289,14 +295,17 @@ def apply_ago_rotations_axes(q, k, rotary_params, positions, sections):
     else:
         if any(isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k)):
             raise ValueError("a differentiable rotation needs CUDA tensors")
-        axis_arguments(rotary_params, positions, sections, dim, _axis_shape(q, positions), None)
+        axis_arguments(rotary_params, positions, sections, dim, _axis_shape(q, positions), None)  # before any copy
         st = Staged(*(t for t in (q, k) if t is not None))
         qt, kt = st.tensors[0], (st.tensors[1] if k is not None else None)
-    if qt.dtype not in _TORCH_DTYPES.values():
+    if qt.dtype not in _TABLE_DTYPES:
         raise TypeError("q and k must be float32, bfloat16 or float64")
     axes = axis_arguments(rotary_params, positions, sections, dim, _axis_shape(qt, positions), qt.device)
-    outs = _RotateAxes.apply(qt, kt, *axes, False)
-    outs = (outs, None) if kt is None else outs
+    if torch.is_grad_enabled() and (qt.requires_grad or (kt is not None and kt.requires_grad)):
+        outs = _RotateAxes.apply(qt, kt, *axes, False)
+        outs = (outs, None) if kt is None else outs
+    else:
+        outs = _rotate_axes(qt, kt, axes, False)
     return tuple(outs) if st is None else (st.back(outs[0]), st.back(outs[1]))
 
 

@@ -51,9 +51,8 @@ struct RowArgs {
   const void* positions;  // [axis][batch][token], strides p_a, p_b, p_t
   const long long* slots;
   long long p_a, p_b, p_t;
-  long long items;        // (batch * tokens) x groups of all sets x chunks of a row
   long long rows;         // cache rows: pages << page_shift
-  int pos64, batch, tokens, D, table_len, page_shift, groups, backward;
+  int pos64, batch, tokens, D, table_len, page_shift, groups, backward, table_runs;
   int end[kMaxAxes];      // pairs [end[a-1], end[a]) belong to axis a; unused axes end at the last
 };
 
@@ -66,78 +65,101 @@ template <typename A> __device__ __forceinline__ A not_a_number();
 template <> __device__ __forceinline__ float not_a_number<float>() { return __int_as_float(0x7fffffff); }
 template <> __device__ __forceinline__ double not_a_number<double>() { return __longlong_as_double(0x7fffffffffffffffll); }
 
+template <typename TT, int P>
+struct alignas(sizeof(TT) * P < 16 ? sizeof(TT) * P : 16) TableRun {
+  TT x[P];
+};
+
 // E elements (E / 2 channel pairs) of a row per thread: 16 bytes, or one pair
-// when rows are not 16-byte aligned.
+// when rows are not 16-byte aligned. Consecutive threads take the chunks of a
+// row and then the next token, so that a warp's accesses are contiguous where
+// rows of a head follow each other (the attention layout), and whole rows
+// otherwise; blockIdx.y is a group of kHeadsPerThread heads of one of the sets.
 template <typename T, typename TT, typename A, int E, typename V>
 __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const __grid_constant__ RowArgs a) {
   constexpr int P = E / 2;
   const int chunks = a.D / E, pairs = a.D / 2;
-  for (long long it = static_cast<long long>(blockIdx.x) * kRowThreads + threadIdx.x; it < a.items;
-       it += static_cast<long long>(gridDim.x) * kRowThreads) {
-    const long long rest = it / chunks;
-    const int e0 = static_cast<int>(it - rest * chunks) * E;
-    const long long row = rest / a.groups;
-    int group = static_cast<int>(rest - row * a.groups);
-    int si = 0;
+  const int idx = blockIdx.x * kRowThreads + threadIdx.x;
+  const int t = idx / chunks;
+  if (t >= a.tokens) return;
+  const int e0 = (idx - t * chunks) * E, p0 = e0 / 2;
+  int group = blockIdx.y, si = 0;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (si == i && i + 1 < a.sets && group >= a.set[i].groups) {
-        group -= a.set[i].groups;
-        ++si;
-      }
-    const RowSet& S = a.set[si];
-    const int b = static_cast<int>(row / a.tokens);
-    const long long t = row - static_cast<long long>(b) * a.tokens;
+  for (int i = 0; i < 2; ++i)
+    if (si == i && i + 1 < a.sets && group >= a.set[i].groups) {
+      group -= a.set[i].groups;
+      ++si;
+    }
+  const RowSet& S = a.set[si];
+  const int h0 = group * kHeadsPerThread;
+  const int end = a.end[kMaxAxes - 1];  // pairs from here on are not turned
+  for (int b = blockIdx.z; b < a.batch; b += gridDim.z) {
     long long at = 0;
-    bool store = true;
     if (S.cache) {
-      const long long slot = a.slots[row];
-      store = slot >= 0 && slot < a.rows;
-      if (!store) continue;
+      const long long slot = a.slots[t];
+      if (slot < 0 || slot >= a.rows) return;
       at = (slot >> a.page_shift) * S.d_b + (slot & ((1 << a.page_shift) - 1)) * S.d_t;
     } else {
       at = b * S.d_b + t * S.d_t;
     }
-    A cc[P], ss[P];
-    if (S.turn) {
-#pragma unroll
-      for (int p = 0; p < P; ++p) {
-        const int pair = e0 / 2 + p;
-        if (pair < a.end[kMaxAxes - 1]) {
-          const int axis = (pair >= a.end[0]) + (pair >= a.end[1]) + (pair >= a.end[2]);
-          const long long m = load_index(a.positions, axis * a.p_a + b * a.p_b + t * a.p_t, a.pos64);
-          const bool in = m >= 0 && m < a.table_len;
-          const long long i = m * pairs + pair;
-          cc[p] = in ? static_cast<A>(to_acc(static_cast<const TT*>(a.c)[i])) : not_a_number<A>();
-          ss[p] = in ? static_cast<A>(to_acc(static_cast<const TT*>(a.s)[i])) : not_a_number<A>();
-          if (a.backward) ss[p] = -ss[p];
-        }
-      }
-    }
     const T* src = static_cast<const T*>(S.src) + b * S.s_b + t * S.s_t + e0;
     T* dst = static_cast<T*>(S.dst) + at + e0;
-    const int h0 = group * kHeadsPerThread;
     V in[kHeadsPerThread];
 #pragma unroll
     for (int j = 0; j < kHeadsPerThread; ++j)
       if (h0 + j < S.heads) in[j] = *reinterpret_cast<const V*>(src + (h0 + j) * S.s_h);
+    if (S.turn && p0 < end) {
+      auto axis_of = [&](int pair) { return (pair >= a.end[0]) + (pair >= a.end[1]) + (pair >= a.end[2]); };
+      auto position = [&](int axis) {
+        return load_index(a.positions, axis * a.p_a + b * a.p_b + t * a.p_t, a.pos64);
+      };
+      A cc[P], ss[P];
+      const int first = axis_of(p0);
+      if (P > 1 && a.table_runs && p0 + P <= end && axis_of(p0 + P - 1) == first) {
+        // The usual case: all pairs of the chunk belong to one axis.
+        const long long m = position(first);
+        if (m >= 0 && m < a.table_len) {
+          const auto cr = *reinterpret_cast<const TableRun<TT, P>*>(static_cast<const TT*>(a.c) + m * pairs + p0);
+          const auto sr = *reinterpret_cast<const TableRun<TT, P>*>(static_cast<const TT*>(a.s) + m * pairs + p0);
 #pragma unroll
-    for (int j = 0; j < kHeadsPerThread; ++j) {
-      if (h0 + j >= S.heads) break;
-      if (S.turn) {
+          for (int p = 0; p < P; ++p) {
+            cc[p] = static_cast<A>(to_acc(cr.x[p]));
+            ss[p] = static_cast<A>(to_acc(sr.x[p]));
+          }
+        } else {
+#pragma unroll
+          for (int p = 0; p < P; ++p) cc[p] = ss[p] = not_a_number<A>();
+        }
+      } else {
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          if (p0 + p >= end) continue;
+          const long long m = position(axis_of(p0 + p));
+          const bool in_table = m >= 0 && m < a.table_len;
+          const long long i = m * pairs + p0 + p;
+          cc[p] = in_table ? static_cast<A>(to_acc(static_cast<const TT*>(a.c)[i])) : not_a_number<A>();
+          ss[p] = in_table ? static_cast<A>(to_acc(static_cast<const TT*>(a.s)[i])) : not_a_number<A>();
+        }
+      }
+      const A sign = a.backward ? A(-1) : A(1);
+#pragma unroll
+      for (int j = 0; j < kHeadsPerThread; ++j) {
         T x[E];
         memcpy(x, &in[j], sizeof(V));
 #pragma unroll
         for (int p = 0; p < P; ++p) {
+          if (p0 + p >= end) continue;
           const A x0 = static_cast<A>(to_acc(x[2 * p])), x1 = static_cast<A>(to_acc(x[2 * p + 1]));
-          if (e0 / 2 + p >= a.end[kMaxAxes - 1]) continue;  // no axis turns it
-          x[2 * p] = from_acc<T>(cc[p] * x0 - ss[p] * x1);
-          x[2 * p + 1] = from_acc<T>(ss[p] * x0 + cc[p] * x1);
+          const A s = sign * ss[p];
+          x[2 * p] = from_acc<T>(cc[p] * x0 - s * x1);
+          x[2 * p + 1] = from_acc<T>(s * x0 + cc[p] * x1);
         }
         memcpy(&in[j], x, sizeof(V));
       }
-      *reinterpret_cast<V*>(dst + (h0 + j) * S.d_h) = in[j];
     }
+#pragma unroll
+    for (int j = 0; j < kHeadsPerThread; ++j)
+      if (h0 + j < S.heads) *reinterpret_cast<V*>(dst + (h0 + j) * S.d_h) = in[j];
   }
 }
 
@@ -149,14 +171,19 @@ template <> struct Pair<double> { using type = uint4; };
 template <typename T, typename TT, typename A>
 cudaError_t launch_rows_tt(RowArgs a, bool wide, cudaStream_t stream) {
   constexpr int E = 16 / sizeof(T);
-  a.items = static_cast<long long>(a.batch) * a.tokens * a.groups * (a.D / (wide ? E : 2));
-  if (a.items == 0) return cudaSuccess;
-  long long blocks = (a.items + kRowThreads - 1) / kRowThreads;
-  if (blocks > 148LL * 64) blocks = 148LL * 64;
+  if (a.batch == 0 || a.tokens == 0) return cudaSuccess;
+  const long long items = static_cast<long long>(a.tokens) * (a.D / (wide ? E : 2));
+  if (items > INT_MAX - kRowThreads || a.groups > 65535) return cudaErrorInvalidConfiguration;
+  const dim3 grid(static_cast<unsigned>((items + kRowThreads - 1) / kRowThreads), a.groups,
+                  a.batch < 65535 ? a.batch : 65535);
+  // A chunk's table values in one or two loads, where its run of pairs is aligned.
+  const size_t run = sizeof(TT) * (E / 2) < 16 ? sizeof(TT) * (E / 2) : 16;
+  a.table_runs = (a.D / 2) % (E / 2) == 0 && reinterpret_cast<uintptr_t>(a.c) % run == 0 &&
+                 reinterpret_cast<uintptr_t>(a.s) % run == 0;
   if (wide)
-    paged_rows_kernel<T, TT, A, E, uint4><<<static_cast<int>(blocks), kRowThreads, 0, stream>>>(a);
+    paged_rows_kernel<T, TT, A, E, uint4><<<grid, kRowThreads, 0, stream>>>(a);
   else
-    paged_rows_kernel<T, TT, A, 2, typename Pair<T>::type><<<static_cast<int>(blocks), kRowThreads, 0, stream>>>(a);
+    paged_rows_kernel<T, TT, A, 2, typename Pair<T>::type><<<grid, kRowThreads, 0, stream>>>(a);
   return cudaGetLastError();
 }
 

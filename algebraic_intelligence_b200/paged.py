@@ -22,8 +22,6 @@ The caches, the block table and the free stack are updated in place.
 """
 from __future__ import annotations
 
-import contextlib
-import ctypes
 from typing import NamedTuple, Optional
 
 import torch
@@ -55,7 +53,7 @@ def _check_page_size(page_size) -> None:
 def _ints(name, t, shape):
     if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
         raise TypeError(f"{name} must be an int32 tensor")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
@@ -71,10 +69,6 @@ def _one_device(*tensors):
             raise ValueError(f"tensors on different devices: {dev} and {t.device}")
         dev = t.device
     return dev
-
-
-def _on(dev):
-    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
 def _no_gradient(what, *tensors):
@@ -103,10 +97,6 @@ def _caches(k_cache, v_cache, ndims=(4,)):
 def _rows(t):
     """A tensor whose last axis is contiguous."""
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
-
-
-def _ll(*values):
-    return (ctypes.c_longlong * len(values))(*values)
 
 
 def paged_plan(block_table, page_counts, seq_lens, new_lens, free_pages, free_count, page_size: int, max_tokens: int,
@@ -160,22 +150,22 @@ def paged_plan(block_table, page_counts, seq_lens, new_lens, free_pages, free_co
     dev = _one_device(block_table, page_counts, seq_lens, new_lens, free_pages, free_count, parents)
     page_counts, seq_lens, new_lens = page_counts.contiguous(), seq_lens.contiguous(), new_lens.contiguous()
     parents = parents.contiguous() if parents is not None else None
-    slots = torch.empty(max_tokens, dtype=torch.int64, device=dev)
-    per_token = torch.empty((2, max_tokens), dtype=torch.int32, device=dev)
-    per_request = torch.empty(3 * b + 2, dtype=torch.int32, device=dev)
-    cu, lens_out, held_out, free_out = per_request.split((b + 1, b, b, 1))
-    rows, positions = per_token[0], per_token[1]
-    granted = torch.empty(b, dtype=torch.bool, device=dev)
-    ancestors = torch.empty((max_tokens, (nodes + 31) // 32), dtype=torch.int32, device=dev) if nodes else None
-    with _on(dev):
-        rc = _lib.load().afa_paged_plan(
-            block_table.data_ptr(), page_counts.data_ptr(), seq_lens.data_ptr(), new_lens.data_ptr(),
-            free_pages.data_ptr(), free_count.data_ptr(), parents.data_ptr() if nodes else None, slots.data_ptr(),
-            rows.data_ptr(), positions.data_ptr(), cu.data_ptr(), lens_out.data_ptr(), held_out.data_ptr(),
-            free_out.data_ptr(), granted.data_ptr(), ancestors.data_ptr() if nodes else None, b, cols, page_size,
-            free_pages.numel(), max_tokens, nodes, _lib.stream_ptr(dev))
+    # One allocation, cut up: int64 slots first, then 32-bit words.
+    words = (nodes + 31) // 32
+    sizes = (2 * max_tokens, max_tokens, max_tokens, b + 1, b, b, 1, max_tokens * words, (b + 3) // 4)
+    buf = torch.empty(sum(sizes), dtype=torch.int32, device=dev)
+    slots, rows, positions, cu, lens_out, held_out, free_out, ancestors, granted = buf.split_with_sizes(sizes)
+    base, at = buf.data_ptr(), [0]
+    for n in sizes:
+        at.append(at[-1] + 4 * n)
+    rc = _lib.call(
+        dev, _lib.load().afa_paged_plan, block_table.data_ptr(), page_counts.data_ptr(), seq_lens.data_ptr(),
+        new_lens.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), parents.data_ptr() if nodes else None,
+        *(base + x for x in at[:7]), base + at[8], base + at[7], b, cols, page_size, free_pages.shape[0], max_tokens,
+        nodes)
     _lib.check(rc, "afa_paged_plan")
-    return PagedPlan(slots, rows, positions, cu, lens_out, held_out, free_out, granted, ancestors)
+    return PagedPlan(slots.view(torch.int64), rows, positions, cu, lens_out, held_out, free_out,
+                     granted.view(torch.bool)[:b], ancestors.view(max_tokens, words) if nodes else None)
 
 
 def paged_append(k, v, k_cache, v_cache, slots, q=None, rotary_params=None, positions=None, sections=None):
@@ -222,17 +212,16 @@ def paged_append(k, v, k_cache, v_cache, slots, q=None, rotary_params=None, posi
     if axes is not None:
         p = axes.positions
         pos = (axes.c.data_ptr(), axes.s.data_ptr(), _lib.dtype_code(axes.c.dtype), axes.c.shape[0], p.data_ptr(),
-               _ll(p.stride(0), p.stride(1)), int(p.dtype == torch.int64), axes.sections, p.shape[0])
+               _lib.longs(p.stride(0), p.stride(1)), int(p.dtype == torch.int64), axes.sections, p.shape[0])
     else:
         pos = (None, None, 0, 0, None, None, 0, None, 0)
-    with _on(dev):
-        rc = _lib.load().afa_paged_append(
-            k.data_ptr(), _ll(k.stride(0), k.stride(1)), v.data_ptr(), _ll(v.stride(0), v.stride(1)),
-            k_cache.data_ptr(), _ll(*k_cache.stride()[:3]), v_cache.data_ptr(), _ll(*v_cache.stride()[:3]),
-            slots.data_ptr(), None if q is None else q.data_ptr(),
-            None if q is None else _ll(q.stride(0), q.stride(1)), None if out is None else out.data_ptr(),
-            0 if q is None else q.shape[1], *pos, tokens, heads, dim, pages, page_size,
-            _lib.dtype_code(k_cache.dtype), _lib.stream_ptr(dev))
+    rc = _lib.call(
+        dev, _lib.load().afa_paged_append, k.data_ptr(), _lib.longs(k.stride(0), k.stride(1)), v.data_ptr(), _lib.longs(v.stride(0), v.stride(1)),
+        k_cache.data_ptr(), _lib.longs(*k_cache.stride()[:3]), v_cache.data_ptr(), _lib.longs(*v_cache.stride()[:3]),
+        slots.data_ptr(), None if q is None else q.data_ptr(),
+        None if q is None else _lib.longs(q.stride(0), q.stride(1)), None if out is None else out.data_ptr(),
+        0 if q is None else q.shape[1], *pos, tokens, heads, dim, pages, page_size,
+        _lib.dtype_code(k_cache.dtype))
     _lib.check(rc, "afa_paged_append")
     return out
 
@@ -309,15 +298,13 @@ def afa_paged(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, ancestors=N
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
     elif not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < need:
         raise ValueError(f"workspace must be a contiguous tensor of at least {need} bytes")
-    with _on(dev):
-        rc = lib.afa_paged(
-            q.data_ptr(), _ll(q.stride(0), q.stride(1)), k_cache.data_ptr(), v_cache.data_ptr(),
-            _ll(*k_cache.stride()[:3]), _ll(*v_cache.stride()[:3]), out.data_ptr(),
-            None if den is None else den.data_ptr(), block_table.data_ptr(), block_table.stride(0),
-            seq_lens.data_ptr(), cu_tokens.data_ptr(), ancestors.data_ptr() if words else None,
-            ancestors.stride(0) if words else 0, words, b, tokens, heads, kv_heads, dim, cols, page_size, pages, code,
-            float(sink_omega), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-            _lib.stream_ptr(dev))
+    rc = _lib.call(
+        dev, lib.afa_paged, q.data_ptr(), _lib.longs(q.stride(0), q.stride(1)), k_cache.data_ptr(), v_cache.data_ptr(),
+        _lib.longs(*k_cache.stride()[:3]), _lib.longs(*v_cache.stride()[:3]), out.data_ptr(),
+        None if den is None else den.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+        seq_lens.data_ptr(), cu_tokens.data_ptr(), ancestors.data_ptr() if words else None,
+        ancestors.stride(0) if words else 0, words, b, tokens, heads, kv_heads, dim, cols, page_size, pages, code,
+        float(sink_omega), workspace.data_ptr(), workspace.numel() * workspace.element_size())
     _lib.check(rc, "afa_paged")
     return (out, den) if return_denominator else out
 
@@ -355,11 +342,10 @@ def paged_commit(k_cache, v_cache, block_table, base_lens, seq_lens, accepted) -
     lens = torch.empty(b, dtype=torch.int32, device=dev)
     layers = k_cache.shape[0] if k_cache.ndim == 5 else 1
     strides = [(0, *t.stride()[:3]) if t.ndim == 4 else t.stride()[:4] for t in (k_cache, v_cache)]
-    with _on(dev):
-        rc = _lib.load().afa_paged_commit(
-            k_cache.data_ptr(), _ll(*strides[0]), v_cache.data_ptr(), _ll(*strides[1]), block_table.data_ptr(),
-            block_table.stride(0), base_lens.data_ptr(), seq_lens.data_ptr(), accepted.data_ptr(),
-            accepted.stride(0) if path else 0, lens.data_ptr(), b, path, layers, heads, dim, cols, pages, page_size,
-            _lib.dtype_code(k_cache.dtype), _lib.stream_ptr(dev))
+    rc = _lib.call(
+        dev, _lib.load().afa_paged_commit, k_cache.data_ptr(), _lib.longs(*strides[0]), v_cache.data_ptr(), _lib.longs(*strides[1]), block_table.data_ptr(),
+        block_table.stride(0), base_lens.data_ptr(), seq_lens.data_ptr(), accepted.data_ptr(),
+        accepted.stride(0) if path else 0, lens.data_ptr(), b, path, layers, heads, dim, cols, pages, page_size,
+        _lib.dtype_code(k_cache.dtype))
     _lib.check(rc, "afa_paged_commit")
     return lens
