@@ -32,6 +32,7 @@ namespace {
 constexpr int kMaxAxes = 4;
 constexpr int kHeadsPerThread = 4;
 constexpr int kRowThreads = 256;
+constexpr int kRowCtas = 148 * 4;  // resident at once
 
 // One of the row sets of a launch: heads x D of every token, from src to dst.
 struct RowSet {
@@ -74,46 +75,24 @@ struct alignas(sizeof(TT) * P < 16 ? sizeof(TT) * P : 16) TableRun {
 // when rows are not 16-byte aligned. Consecutive threads take the chunks of a
 // row and then the next token, so that a warp's accesses are contiguous where
 // rows of a head follow each other (the attention layout), and whole rows
-// otherwise; blockIdx.y is a group of kHeadsPerThread heads of one of the sets.
+// otherwise. A thread reads its cosines and sines once and walks every
+// gridDim.y-th group of kHeadsPerThread heads, whose loads go out together.
 template <typename T, typename TT, typename A, int E, typename V>
-__global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const __grid_constant__ RowArgs a) {
+__global__ void __launch_bounds__(kRowThreads, 4) paged_rows_kernel(const __grid_constant__ RowArgs a) {
   constexpr int P = E / 2;
   const int chunks = a.D / E, pairs = a.D / 2;
   const int idx = blockIdx.x * kRowThreads + threadIdx.x;
   const int t = idx / chunks;
   if (t >= a.tokens) return;
   const int e0 = (idx - t * chunks) * E, p0 = e0 / 2;
-  int group = blockIdx.y, si = 0;
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if (si == i && i + 1 < a.sets && group >= a.set[i].groups) {
-      group -= a.set[i].groups;
-      ++si;
-    }
-  const RowSet& S = a.set[si];
-  const int h0 = group * kHeadsPerThread;
   const int end = a.end[kMaxAxes - 1];  // pairs from here on are not turned
   for (int b = blockIdx.z; b < a.batch; b += gridDim.z) {
-    long long at = 0;
-    if (S.cache) {
-      const long long slot = a.slots[t];
-      if (slot < 0 || slot >= a.rows) return;
-      at = (slot >> a.page_shift) * S.d_b + (slot & ((1 << a.page_shift) - 1)) * S.d_t;
-    } else {
-      at = b * S.d_b + t * S.d_t;
-    }
-    const T* src = static_cast<const T*>(S.src) + b * S.s_b + t * S.s_t + e0;
-    T* dst = static_cast<T*>(S.dst) + at + e0;
-    V in[kHeadsPerThread];
-#pragma unroll
-    for (int j = 0; j < kHeadsPerThread; ++j)
-      if (h0 + j < S.heads) in[j] = *reinterpret_cast<const V*>(src + (h0 + j) * S.s_h);
-    if (S.turn && p0 < end) {
+    A cc[P], ss[P];
+    if (p0 < end) {
       auto axis_of = [&](int pair) { return (pair >= a.end[0]) + (pair >= a.end[1]) + (pair >= a.end[2]); };
       auto position = [&](int axis) {
         return load_index(a.positions, axis * a.p_a + b * a.p_b + t * a.p_t, a.pos64);
       };
-      A cc[P], ss[P];
       const int first = axis_of(p0);
       if (P > 1 && a.table_runs && p0 + P <= end && axis_of(p0 + P - 1) == first) {
         // The usual case: all pairs of the chunk belong to one axis.
@@ -141,25 +120,56 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const __grid_co
           ss[p] = in_table ? static_cast<A>(to_acc(static_cast<const TT*>(a.s)[i])) : not_a_number<A>();
         }
       }
-      const A sign = a.backward ? A(-1) : A(1);
+      if (a.backward) {
 #pragma unroll
-      for (int j = 0; j < kHeadsPerThread; ++j) {
-        T x[E];
-        memcpy(x, &in[j], sizeof(V));
-#pragma unroll
-        for (int p = 0; p < P; ++p) {
-          if (p0 + p >= end) continue;
-          const A x0 = static_cast<A>(to_acc(x[2 * p])), x1 = static_cast<A>(to_acc(x[2 * p + 1]));
-          const A s = sign * ss[p];
-          x[2 * p] = from_acc<T>(cc[p] * x0 - s * x1);
-          x[2 * p + 1] = from_acc<T>(s * x0 + cc[p] * x1);
-        }
-        memcpy(&in[j], x, sizeof(V));
+        for (int p = 0; p < P; ++p) ss[p] = -ss[p];
       }
     }
+    for (int x = blockIdx.y; x < a.groups; x += gridDim.y) {
+      int group = x, si = 0;
 #pragma unroll
-    for (int j = 0; j < kHeadsPerThread; ++j)
-      if (h0 + j < S.heads) *reinterpret_cast<V*>(dst + (h0 + j) * S.d_h) = in[j];
+      for (int i = 0; i < 2; ++i)
+        if (si == i && i + 1 < a.sets && group >= a.set[i].groups) {
+          group -= a.set[i].groups;
+          ++si;
+        }
+      const RowSet& S = a.set[si];
+      long long at = 0;
+      if (S.cache) {
+        const long long slot = a.slots[t];
+        if (slot < 0 || slot >= a.rows) continue;
+        at = (slot >> a.page_shift) * S.d_b + (slot & ((1 << a.page_shift) - 1)) * S.d_t;
+      } else {
+        at = b * S.d_b + t * S.d_t;
+      }
+      const int h0 = group * kHeadsPerThread, nh = S.heads - h0;
+      const T* src = static_cast<const T*>(S.src) + b * S.s_b + t * S.s_t + h0 * S.s_h + e0;
+      T* dst = static_cast<T*>(S.dst) + at + h0 * S.d_h + e0;
+      V in[kHeadsPerThread];
+#pragma unroll
+      for (int j = 0; j < kHeadsPerThread; ++j) {
+        if (j < nh) in[j] = *reinterpret_cast<const V*>(src);
+        src += S.s_h;
+      }
+      const bool turn = S.turn && p0 < end;
+#pragma unroll
+      for (int j = 0; j < kHeadsPerThread; ++j) {
+        if (turn) {
+          T y[E];
+          memcpy(y, &in[j], sizeof(V));
+#pragma unroll
+          for (int p = 0; p < P; ++p) {
+            if (p0 + p >= end) continue;
+            const A x0 = static_cast<A>(to_acc(y[2 * p])), x1 = static_cast<A>(to_acc(y[2 * p + 1]));
+            y[2 * p] = from_acc<T>(cc[p] * x0 - ss[p] * x1);
+            y[2 * p + 1] = from_acc<T>(ss[p] * x0 + cc[p] * x1);
+          }
+          memcpy(&in[j], y, sizeof(V));
+        }
+        if (j < nh) *reinterpret_cast<V*>(dst) = in[j];
+        dst += S.d_h;
+      }
+    }
   }
 }
 
@@ -173,9 +183,12 @@ cudaError_t launch_rows_tt(RowArgs a, bool wide, cudaStream_t stream) {
   constexpr int E = 16 / sizeof(T);
   if (a.batch == 0 || a.tokens == 0) return cudaSuccess;
   const long long items = static_cast<long long>(a.tokens) * (a.D / (wide ? E : 2));
-  if (items > INT_MAX - kRowThreads || a.groups > 65535) return cudaErrorInvalidConfiguration;
-  const dim3 grid(static_cast<unsigned>((items + kRowThreads - 1) / kRowThreads), a.groups,
-                  a.batch < 65535 ? a.batch : 65535);
+  if (items > INT_MAX - kRowThreads) return cudaErrorInvalidConfiguration;
+  // Heads are spread over CTAs as far as it takes to have kRowCtas of them.
+  const long long x = (items + kRowThreads - 1) / kRowThreads, z = a.batch < 65535 ? a.batch : 65535;
+  long long y = (kRowCtas + x * z - 1) / (x * z);
+  if (y > a.groups) y = a.groups;
+  const dim3 grid(static_cast<unsigned>(x), static_cast<unsigned>(y), static_cast<unsigned>(z));
   // A chunk's table values in one or two loads, where its run of pairs is aligned.
   const size_t run = sizeof(TT) * (E / 2) < 16 ? sizeof(TT) * (E / 2) : 16;
   a.table_runs = (a.D / 2) % (E / 2) == 0 && reinterpret_cast<uintptr_t>(a.c) % run == 0 &&
