@@ -17,6 +17,7 @@
 // dimensions the tensor-core kernel (afa_paged_tc.cu) does not take, the kernel
 // that adds fragments, and the C entry point. The work split is in
 // afa_paged.cuh.
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <cstdio>
@@ -29,33 +30,70 @@
 namespace afa {
 namespace {
 
-constexpr int kSimtRows = 32;
 constexpr int kSimtThreads = 256;
 
-// 32 query rows x BN keys per step, 16 x 16 threads; thread (ty, tx) owns
-// scores (ty + 16 i, tx + 16 j) and outputs (ty + 16 i, tx + 16 j'), so that
-// shared-memory reads (row pitch DMAX + 1) are free of bank conflicts. Sums run
-// over BN keys in registers of their own before they join the row's, which
-// keeps float32 results near 1e-7 at any length.
-template <typename T, typename A, int BN, int DMAX>
+// 16 bytes of accumulators.
+template <typename A>
+struct alignas(16) Quad {
+  static constexpr int N = 16 / sizeof(A);
+  A x[N];
+};
+
+// ROWS query rows x BN keys per step. 256 threads as RY x CX: thread (ty, tx)
+// owns scores (ty + RY i, tx + CX j) and, of outputs, the channels of 16 bytes
+// number tx + CX j of the same rows. Shared memory holds rows of DMAX padded by
+// 16 bytes, read 16 bytes at a time: a quarter warp's reads fall on different
+// banks or are one broadcast. Bound by those reads and the FMAs (8 or 32 rows
+// share every key); several CTAs per SM cover the loads' latency. Sums run over
+// BN keys in registers of their own before they join the row's, which keeps
+// float32 results near 1e-7 at any length.
+template <typename T, typename A, int ROWS, int BN, int DMAX>
+struct SimtCfg {
+  static constexpr int RY = ROWS < 16 ? ROWS : 16, CX = kSimtThreads / RY;
+  static constexpr int TR = ROWS / RY, TC = BN / CX;
+  static constexpr int V = Quad<A>::N;
+  static constexpr int LD = DMAX + V, PLD = BN + V;
+  static constexpr int OC = (DMAX / V + CX - 1) / CX;
+  static constexpr size_t kSmem = sizeof(A) * (static_cast<size_t>(ROWS + 2 * BN) * LD + static_cast<size_t>(ROWS) * PLD);
+};
+
+template <typename T, typename A, int ROWS, int BN, int DMAX>
 __global__ void __launch_bounds__(kSimtThreads) afa_paged_simt_kernel(const __grid_constant__ PagedArgs a) {
-  constexpr int LD = DMAX + 1, PLD = BN + 1, TR = kSimtRows / 16, TC = BN / 16, OC = DMAX / 16;
+  using C = SimtCfg<T, A, ROWS, BN, DMAX>;
+  constexpr int RY = C::RY, CX = C::CX, TR = C::TR, TC = C::TC, V = C::V, LD = C::LD, PLD = C::PLD, OC = C::OC;
+  using Q4 = Quad<A>;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   __shared__ long long share_sm[kSimtThreads / 32 + 4];
-  __shared__ unsigned char in_cache[BN];
+  __shared__ long long k_row[BN], v_row[BN];  // offsets of the step's cache rows; below 0: none
   A* Qs = reinterpret_cast<A*>(smem_raw);
-  A* Ks = Qs + kSimtRows * LD;
+  A* Ks = Qs + ROWS * LD;
   A* Vs = Ks + BN * LD;
   A* Ps = Vs + BN * LD;
-  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, D = a.D;
+  const int tid = threadIdx.x, tx = tid % CX, ty = tid / CX, D = a.D;
+  const int dv = (D + V - 1) / V;  // 16-byte channel groups; the last is padded with zeros
   const T* q = static_cast<const T*>(a.q);
-  const T* k = static_cast<const T*>(a.k);
-  const T* v = static_cast<const T*>(a.v);
   T* out = static_cast<T*>(a.out);
   A* dtot = static_cast<A*>(a.dtot);
   const A scale = sizeof(A) == 8 ? static_cast<A>(a.scale_d) : static_cast<A>(a.scale);
   const A sink = sizeof(A) == 8 ? static_cast<A>(a.sink_d) : static_cast<A>(a.sink);
   A* frag = static_cast<A*>(a.frag) + static_cast<long long>(blockIdx.x) * 2 * a.frag_rows * (D + 1);
+  // One group of channels of a row (zeros where p is null), in the accumulators' type.
+  auto fetch = [&](const T* p, int c) {
+    Q4 r;
+    const int c0 = c * V;
+    if (p && a.wide) {
+      struct alignas(V * sizeof(T)) Run {
+        T x[V];
+      };
+      const Run w = *reinterpret_cast<const Run*>(p + c0);
+#pragma unroll
+      for (int e = 0; e < V; ++e) r.x[e] = static_cast<A>(to_acc(w.x[e]));
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) r.x[e] = p && c0 + e < D ? static_cast<A>(to_acc(p[c0 + e])) : A(0);
+    }
+    return r;
+  };
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // see paged_combine_kernel
   PagedWalk walk;
@@ -63,49 +101,60 @@ __global__ void __launch_bounds__(kSimtThreads) afa_paged_simt_kernel(const __gr
   if (tid == 0) paged_meta_clear(a.meta);
   PagedPiece p;
   while (walk.next(a, p)) {
-    const long long row0 = static_cast<long long>(p.u) * kSimtRows;
-    const int rows = static_cast<int>(min(static_cast<long long>(kSimtRows), static_cast<long long>(p.r.n) * a.G - row0));
+    const int row0 = p.u * ROWS;
+    const int rows = min(ROWS, p.r.n * a.G - row0);
     if (tid == 0) paged_meta_piece(a.meta, p);
     __syncthreads();
-    for (int i = tid; i < kSimtRows * D; i += kSimtThreads) {
-      const int r = i / D, c = i - r * D;
-      A x = A(0);
+    for (int i = tid; i < ROWS * dv; i += kSimtThreads) {
+      const int r = i / dv, c = i - r * dv;
+      const T* src = nullptr;
       if (r < rows) {
-        const long long row = row0 + r;
-        const long long tok = row / a.G;
-        const int g = static_cast<int>(row - tok * a.G);
-        x = static_cast<A>(to_acc(q[(p.r.tok0 + tok) * a.q_st + (static_cast<long long>(p.h) * a.G + g) * a.q_sh + c]));
+        const int tok = (row0 + r) / a.G, g = row0 + r - tok * a.G;
+        src = q + (static_cast<long long>(p.r.tok0) + tok) * a.q_st + (static_cast<long long>(p.h) * a.G + g) * a.q_sh;
       }
-      Qs[r * LD + c] = x;
+      *reinterpret_cast<Q4*>(Qs + r * LD + c * V) = fetch(src, c);
     }
     int node[TR];
-    A o[TR][OC], rs[TR];
+    A o[TR][OC][V], rs[TR];
 #pragma unroll
     for (int i = 0; i < TR; ++i) {
-      const int r = ty + 16 * i;
-      node[i] = r < rows ? static_cast<int>((row0 + r) / a.G) : -1;
+      const int r = ty + RY * i;
+      node[i] = r < rows ? (row0 + r) / a.G : -1;
       rs[i] = A(0);
 #pragma unroll
-      for (int j = 0; j < OC; ++j) o[i][j] = A(0);
+      for (int j = 0; j < OC; ++j)
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[i][j][e] = A(0);
     }
-    const int k_end = min(p.t1 * kPagedTile, p.tiles == 0 ? 0 : p.r.len);
+    const int k_end = p.tiles == 0 ? 0 : min(p.t1 * kPagedTile, p.r.len);
+    const int prefix = p.r.len - p.r.n;
     for (int k0 = p.t0 * kPagedTile; k0 < k_end; k0 += BN) {
       __syncthreads();
-      for (int i = tid; i < BN * D; i += kSimtThreads) {
-        const int r = i / D, c = i - r * D, key = k0 + r;
-        A kx = A(0), vx = A(0);
+      bool missing = false;
+      if (tid < BN) {
+        const int key = k0 + tid;
+        long long ko = -1, vo = -1;
         if (key < p.r.len) {
           const int page = a.table[p.b * a.table_ld + (key >> a.page_shift)];
           const long long in = key & ((1 << a.page_shift) - 1);
-          const bool ok = page >= 0 && page < a.num_pages;
-          if (c == 0) in_cache[r] = ok;
-          if (ok) {
-            kx = static_cast<A>(to_acc(k[page * a.k_sp + p.h * a.k_sh + in * a.k_sr + c]));
-            vx = static_cast<A>(to_acc(v[page * a.v_sp + p.h * a.v_sh + in * a.v_sr + c]));
+          if (page >= 0 && page < a.num_pages) {
+            ko = page * a.k_sp + p.h * a.k_sh + in * a.k_sr;
+            vo = page * a.v_sp + p.h * a.v_sh + in * a.v_sr;
           }
         }
-        Ks[r * LD + c] = kx;
-        Vs[r * LD + c] = vx;
+        k_row[tid] = ko;
+        v_row[tid] = vo;
+        missing = ko < 0;
+      }
+      const bool all_seen = !__syncthreads_or(missing) && k0 + BN <= prefix;
+#pragma unroll 4
+      for (int i = tid; i < BN * dv; i += kSimtThreads) {
+        const int r = i / dv, c = i - r * dv;
+        const long long ko = k_row[r], vo = v_row[r];
+        const Q4 kx = fetch(ko < 0 ? nullptr : static_cast<const T*>(a.k) + ko, c);
+        const Q4 vx = fetch(ko < 0 ? nullptr : static_cast<const T*>(a.v) + vo, c);
+        *reinterpret_cast<Q4*>(Ks + r * LD + c * V) = kx;
+        *reinterpret_cast<Q4*>(Vs + r * LD + c * V) = vx;
       }
       __syncthreads();
       A s[TR][TC];
@@ -113,85 +162,102 @@ __global__ void __launch_bounds__(kSimtThreads) afa_paged_simt_kernel(const __gr
       for (int i = 0; i < TR; ++i)
 #pragma unroll
         for (int j = 0; j < TC; ++j) s[i][j] = A(0);
-      for (int d = 0; d < D; ++d) {
-        A x[TR], y[TC];
+#pragma unroll 4
+      for (int c = 0; c < dv; ++c) {
+        Q4 x[TR], y[TC];
 #pragma unroll
-        for (int i = 0; i < TR; ++i) x[i] = Qs[(ty + 16 * i) * LD + d];
+        for (int i = 0; i < TR; ++i) x[i] = *reinterpret_cast<const Q4*>(Qs + (ty + RY * i) * LD + c * V);
 #pragma unroll
-        for (int j = 0; j < TC; ++j) y[j] = Ks[(tx + 16 * j) * LD + d];
+        for (int j = 0; j < TC; ++j) y[j] = *reinterpret_cast<const Q4*>(Ks + (tx + CX * j) * LD + c * V);
 #pragma unroll
-        for (int i = 0; i < TR; ++i)
+        for (int e = 0; e < V; ++e)
 #pragma unroll
-          for (int j = 0; j < TC; ++j) s[i][j] = fma(x[i], y[j], s[i][j]);
+          for (int i = 0; i < TR; ++i)
+#pragma unroll
+            for (int j = 0; j < TC; ++j) s[i][j] = fma(x[i].x[e], y[j].x[e], s[i][j]);
       }
 #pragma unroll
       for (int i = 0; i < TR; ++i) {
         A part = A(0);
 #pragma unroll
         for (int w = 0; w < (BN + 31) / 32; ++w) {
-          const unsigned seen = node[i] < 0 ? 0u : paged_seen(a, p.r, node[i], k0 + 32 * w);
+          const unsigned seen = all_seen ? 0xffffffffu : node[i] < 0 ? 0u : paged_seen(a, p.r, node[i], k0 + 32 * w);
 #pragma unroll
           for (int j = 0; j < TC; ++j) {
-            const int c = tx + 16 * j;
-            if (c / 32 != w) continue;
-            const A pr = ((seen >> (c & 31)) & 1u) && in_cache[c] ? octic_ref(s[i][j] * scale) : A(0);
+            const int c = tx + CX * j;
+            if ((CX * j) / 32 != w) continue;
+            const bool in = ((seen >> (c & 31)) & 1u) && (all_seen || k_row[c] >= 0);
+            const A pr = in ? octic_ref(s[i][j] * scale) : A(0);
             part += pr;
-            Ps[(ty + 16 * i) * PLD + c] = pr;
+            Ps[(ty + RY * i) * PLD + c] = pr;
           }
         }
         rs[i] += part;
       }
       __syncthreads();
-      A ot[TR][OC];
+      A ot[TR][OC][V];
 #pragma unroll
       for (int i = 0; i < TR; ++i)
 #pragma unroll
-        for (int j = 0; j < OC; ++j) ot[i][j] = A(0);
-#pragma unroll 4
-      for (int kk = 0; kk < BN; ++kk) {
-        A pv[TR];
+        for (int j = 0; j < OC; ++j)
 #pragma unroll
-        for (int i = 0; i < TR; ++i) pv[i] = Ps[(ty + 16 * i) * PLD + kk];
+          for (int e = 0; e < V; ++e) ot[i][j][e] = A(0);
+#pragma unroll 2
+      for (int kk = 0; kk < BN; kk += V) {
+        Q4 pv[TR];
+#pragma unroll
+        for (int i = 0; i < TR; ++i) pv[i] = *reinterpret_cast<const Q4*>(Ps + (ty + RY * i) * PLD + kk);
 #pragma unroll
         for (int j = 0; j < OC; ++j) {
-          const int c = tx + 16 * j;
-          if (c < D) {
-            const A vv = Vs[kk * LD + c];
+          const int c = tx + CX * j;
+          if (c < dv) {
 #pragma unroll
-            for (int i = 0; i < TR; ++i) ot[i][j] = fma(pv[i], vv, ot[i][j]);
+            for (int y = 0; y < V; ++y) {
+              const Q4 vv = *reinterpret_cast<const Q4*>(Vs + (kk + y) * LD + c * V);
+#pragma unroll
+              for (int i = 0; i < TR; ++i)
+#pragma unroll
+                for (int e = 0; e < V; ++e) ot[i][j][e] = fma(pv[i].x[y], vv.x[e], ot[i][j][e]);
+            }
           }
         }
       }
 #pragma unroll
       for (int i = 0; i < TR; ++i)
 #pragma unroll
-        for (int j = 0; j < OC; ++j) o[i][j] += ot[i][j];
+        for (int j = 0; j < OC; ++j)
+#pragma unroll
+          for (int e = 0; e < V; ++e) o[i][j][e] += ot[i][j][e];
     }
-    // The 16 threads of a half-warp share their rows.
+    // The CX threads of a row are neighbours in a warp.
 #pragma unroll
     for (int i = 0; i < TR; ++i) {
 #pragma unroll
-      for (int off = 8; off > 0; off >>= 1) rs[i] += __shfl_xor_sync(0xffffffffu, rs[i], off);
-      const int r = ty + 16 * i;
+      for (int off = CX / 2; off > 0; off >>= 1) rs[i] += __shfl_xor_sync(0xffffffffu, rs[i], off);
+      const int r = ty + RY * i;
       if (r >= rows) continue;
-      if (p.whole()) {
-        const long long row = row0 + r, tok = p.r.tok0 + row / a.G;
-        const long long orow = tok * a.Hkv * a.G + static_cast<long long>(p.h) * a.G + row % a.G;
-        const A denom = rs[i] + sink;
+      const int tok = (row0 + r) / a.G;
+      const long long orow = (static_cast<long long>(p.r.tok0) + tok) * a.Hkv * a.G +
+                             static_cast<long long>(p.h) * a.G + (row0 + r - tok * a.G);
+      const bool whole = p.whole();
+      const A denom = rs[i] + sink;
+      A* f = frag + static_cast<long long>(paged_frag_slot(p)) * a.frag_rows * (D + 1);
 #pragma unroll
-        for (int j = 0; j < OC; ++j) {
-          const int c = tx + 16 * j;
-          if (c < D) out[orow * D + c] = from_acc<T>(denom > A(0) ? o[i][j] / denom : A(0));
-        }
-        if (tx == 0 && dtot) dtot[orow] = denom;
-      } else {
-        A* f = frag + static_cast<long long>(paged_frag_slot(p)) * a.frag_rows * (D + 1);
+      for (int j = 0; j < OC; ++j)
 #pragma unroll
-        for (int j = 0; j < OC; ++j) {
-          const int c = tx + 16 * j;
-          if (c < D) f[r * D + c] = o[i][j];
+        for (int e = 0; e < V; ++e) {
+          const int c = (tx + CX * j) * V + e;
+          if (c >= D) continue;
+          if (whole)
+            out[orow * D + c] = from_acc<T>(denom > A(0) ? o[i][j][e] / denom : A(0));
+          else
+            f[static_cast<long long>(r) * D + c] = o[i][j][e];
         }
-        if (tx == 0) f[a.frag_rows * D + r] = rs[i];
+      if (tx == 0) {
+        if (!whole)
+          f[static_cast<long long>(a.frag_rows) * D + r] = rs[i];
+        else if (dtot)
+          dtot[orow] = denom;
       }
     }
   }
@@ -261,12 +327,12 @@ __global__ void __launch_bounds__(kCombineWarps * 32) paged_combine_kernel(const
   }
 }
 
-template <typename T, typename A, int BN, int DMAX>
+template <typename T, typename A, int ROWS, int BN, int DMAX>
 cudaError_t launch_simt(const PagedArgs& a, int ctas, cudaStream_t stream) {
-  constexpr size_t smem = sizeof(A) * (static_cast<size_t>(kSimtRows + 2 * BN) * (DMAX + 1) +
-                                       static_cast<size_t>(kSimtRows) * (BN + 1));
+  constexpr size_t smem = SimtCfg<T, A, ROWS, BN, DMAX>::kSmem;
+  static_assert(smem <= 227 * 1024, "shared memory per CTA");
   static PerDeviceOnce setup;
-  auto kern = afa_paged_simt_kernel<T, A, BN, DMAX>;
+  auto kern = afa_paged_simt_kernel<T, A, ROWS, BN, DMAX>;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess)
@@ -278,16 +344,21 @@ cudaError_t launch_simt(const PagedArgs& a, int ctas, cudaStream_t stream) {
   return cudaGetLastError();
 }
 
+template <typename T, typename A, int ROWS>
+cudaError_t launch_simt_rows(const PagedArgs& a, int ctas, cudaStream_t stream) {
+  if constexpr (sizeof(A) == 8) {
+    if (a.D <= 128) return launch_simt<T, A, ROWS, 32, 128>(a, ctas, stream);
+    return launch_simt<T, A, ROWS, 32, 256>(a, ctas, stream);
+  } else {
+    if (a.D <= 64) return launch_simt<T, A, ROWS, 64, 64>(a, ctas, stream);
+    if (a.D <= 128) return launch_simt<T, A, ROWS, 64, 128>(a, ctas, stream);
+    return launch_simt<T, A, ROWS, 32, 256>(a, ctas, stream);
+  }
+}
+
 template <typename T, typename A>
 cudaError_t launch_simt_type(const PagedArgs& a, int ctas, cudaStream_t stream) {
-  if constexpr (sizeof(A) == 8) {
-    if (a.D <= 128) return launch_simt<T, A, 32, 128>(a, ctas, stream);
-    return launch_simt<T, A, 32, 256>(a, ctas, stream);
-  } else {
-    if (a.D <= 64) return launch_simt<T, A, 64, 64>(a, ctas, stream);
-    if (a.D <= 128) return launch_simt<T, A, 64, 128>(a, ctas, stream);
-    return launch_simt<T, A, 32, 256>(a, ctas, stream);
-  }
+  return a.unit_rows == 8 ? launch_simt_rows<T, A, 8>(a, ctas, stream) : launch_simt_rows<T, A, 32>(a, ctas, stream);
 }
 
 template <typename T, typename A, int W>
@@ -327,24 +398,32 @@ int sm_count() {
   return e == cudaSuccess ? count[dev] : 0;
 }
 
-constexpr int kMaxPagedCtas = 148;
+// CTAs of a launch per SM: one of the tensor-core kernels fills an SM, of the
+// CUDA-core kernel up to four fit (float32, 64 channels).
+constexpr int kMaxSms = 148, kSimtPerSm = 4;
 
-// Query rows per work unit and the workspace layout: meta, then fragments.
-// Sized for the tensor-core kernel's units where it may run.
-int max_unit_rows(int dtype, int G, int D) {
-  return dtype == kBF16 && (D == 64 || D == 128) && G <= 128 ? paged_tc_unit_rows(G) : kSimtRows;
+// Rows of a CUDA-core unit: 8 where requests have no more on average (single
+// tokens), else 32.
+int simt_unit_rows(int B, int T, int G) {
+  return (static_cast<long long>(T) + B - 1) / B * G <= 8 ? 8 : 32;
 }
+
 // A multiple of four, so that fragments start on 16 bytes whatever D is.
 int frag_rows_of(int unit_rows, int T, int G) {
   const long long all = static_cast<long long>(T) * G;
   return ((all < unit_rows ? static_cast<int>(all) : unit_rows) + 3) / 4 * 4;
 }
-constexpr size_t kMetaBytes = (static_cast<size_t>(kMaxPagedCtas) * 4 * sizeof(int) + 255) / 256 * 256;
+
+// Workspace: meta (4 ints per CTA), then two fragments per CTA.
+constexpr size_t kMetaBytes = (static_cast<size_t>(kMaxSms) * kSimtPerSm * 4 * sizeof(int) + 255) / 256 * 256;
 
 size_t workspace_bytes(int T, int Hq, int Hkv, int D, int dtype) {
   const size_t acc = dtype == kF64 ? 8 : 4;
-  const size_t rows = frag_rows_of(max_unit_rows(dtype, Hq / Hkv, D), T, Hq / Hkv);
-  return kMetaBytes + static_cast<size_t>(kMaxPagedCtas) * 2 * rows * (static_cast<size_t>(D) + 1) * acc;
+  const int G = Hq / Hkv;
+  size_t rows = static_cast<size_t>(kMaxSms) * kSimtPerSm * frag_rows_of(32, T, G);
+  if (dtype == kBF16 && (D == 64 || D == 128) && G <= 128)  // the tensor-core kernels may run
+    rows = std::max(rows, static_cast<size_t>(kMaxSms) * frag_rows_of(paged_tc_unit_rows(G), T, G));
+  return kMetaBytes + 2 * rows * (static_cast<size_t>(D) + 1) * acc;
 }
 
 int invalid(const char* msg) { return set_last_error(AFA_ERR_INVALID, msg); }
@@ -378,6 +457,7 @@ extern "C" int afa_paged(const void* q, const long long* q_strides, const void* 
   if (!(std::isfinite(sink_omega) && sink_omega >= 0.f)) return invalid("sink_omega must be finite and nonnegative");
   if (static_cast<long long>(table_cols) * page_size > INT_MAX - 65536)
     return invalid("afa_paged: a block table row may hold at most 2^31 - 65537 tokens");
+  if (static_cast<long long>(tokens) * q_heads > INT_MAX / 2) return invalid("afa_paged: too many query rows");
   if (ancestors && ancestor_words <= 0) return invalid("ancestors needs at least one word per token");
   if (tokens == 0 || batch == 0) return AFA_OK;
   if (!q || !k_cache || !v_cache || !out || !block_table || !seq_lens || !cu_tokens || !q_strides || !k_strides ||
@@ -425,13 +505,21 @@ extern "C" int afa_paged(const void* q, const long long* q_strides, const void* 
   a.meta = static_cast<int*>(workspace);
   a.frag = static_cast<char*>(workspace) + kMetaBytes;
   a.status = device_status_ptr();
-  int ctas = sm_count();
+  int ctas = std::min(sm_count(), kMaxSms);
   if (!a.status || ctas <= 0) return set_last_error(AFA_ERR_CUDA, "afa_paged: device set-up failed");
-  if (ctas > kMaxPagedCtas) ctas = kMaxPagedCtas;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool tc = paged_tc_supported(a, dtype);
   const int nt = tc ? paged_tr_rows(batch, tokens, a.G) : 0;
-  a.unit_rows = nt ? nt / a.G * a.G : tc ? paged_tc_unit_rows(a.G) : kSimtRows;
+  a.unit_rows = nt ? nt / a.G * a.G : tc ? paged_tc_unit_rows(a.G) : simt_unit_rows(batch, tokens, a.G);
+  a.min_share = tc ? 2 : 1;
+  if (!tc) {
+    const size_t es = dtype_size(dtype), run = es * (dtype == kF64 ? 2 : 4);  // a channel group in memory
+    a.wide = static_cast<size_t>(D) * es % run == 0;
+    for (const void* x : {a.q, a.k, a.v}) a.wide = a.wide && reinterpret_cast<uintptr_t>(x) % run == 0;
+    for (long long s : {a.q_st, a.q_sh, a.k_sp, a.k_sh, a.k_sr, a.v_sp, a.v_sh, a.v_sr})
+      a.wide = a.wide && s * static_cast<long long>(es) % static_cast<long long>(run) == 0;
+    ctas *= kSimtPerSm;
+  }
   a.frag_rows = frag_rows_of(a.unit_rows, tokens, a.G);
   const char* detail = "";
   cudaError_t e;

@@ -32,21 +32,20 @@ __device__ __forceinline__ PagedReq paged_req(const PagedArgs& a, int b) {
 }
 
 __device__ __forceinline__ int paged_units(const PagedArgs& a, const PagedReq& r) {
-  return static_cast<int>((static_cast<long long>(r.n) * a.G + a.unit_rows - 1) / a.unit_rows);
+  return (r.n * a.G + a.unit_rows - 1) / a.unit_rows;  // rows of a launch stay below 2^30
 }
 
 // Keys that some row of rows [.., row_end) of a request can see: all of them
 // with a mask of drafted nodes, otherwise those up to the last row's token.
-__device__ __forceinline__ int paged_visible(const PagedArgs& a, const PagedReq& r, long long row_end) {
+__device__ __forceinline__ int paged_visible(const PagedArgs& a, const PagedReq& r, int row_end) {
   if (a.anc) return r.len;
-  const long long rows = static_cast<long long>(r.n) * a.G;
-  const int last = static_cast<int>(((row_end < rows ? row_end : rows) - 1) / a.G);
+  const int last = (min(row_end, r.n * a.G) - 1) / a.G;
   const int vis = r.len - r.n + last + 1;
   return vis < 0 ? 0 : vis;
 }
 
 __device__ __forceinline__ int paged_tiles(const PagedArgs& a, const PagedReq& r, int u) {
-  return (paged_visible(a, r, static_cast<long long>(u + 1) * a.unit_rows) + kPagedTile - 1) / kPagedTile;
+  return (paged_visible(a, r, (u + 1) * a.unit_rows) + kPagedTile - 1) / kPagedTile;
 }
 
 // Cost of a unit: its key tiles; a unit that sees no key still writes its rows.
@@ -71,9 +70,6 @@ struct PagedShare {
   long long left;  // the share's cost
   int ctas;        // CTAs that have a share
 };
-
-// Smallest share: below it the fixed cost of a CTA outweighs the keys it reads.
-constexpr int kPagedMinShare = 2;
 
 // This CTA's share. Called by all NT threads; `sm` is scratch of NT / 32 + 4
 // 8-byte words. Every CTA adds up the requests' costs by itself: it costs less
@@ -104,7 +100,7 @@ __device__ __forceinline__ PagedShare paged_share(const PagedArgs& a, long long*
   }
   const long long first = before + inc - mine;  // cost before this thread's requests
   PagedShare s;
-  const long long most = (total + kPagedMinShare - 1) / kPagedMinShare;
+  const long long most = (total + a.min_share - 1) / a.min_share;
   s.ctas = most < gridDim.x ? static_cast<int>(most) : static_cast<int>(gridDim.x);
   const int c = blockIdx.x;
   if (c >= s.ctas) {
