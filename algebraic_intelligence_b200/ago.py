@@ -216,7 +216,8 @@ def axis_arguments(rotary_params, positions, sections, dim, shape, device) -> Ax
 
 def _row_strides(t, token_major):
     """Strides (batch, token, head) of the rows of t."""
-    return _lib.longs(0, *t.stride()[:2]) if token_major else _lib.longs(*(t.stride(i) for i in (0, 2, 1)))
+    st = t.stride()
+    return _lib.longs(0, st[0], st[1]) if token_major else _lib.longs(st[0], st[2], st[1])
 
 
 def _rotate_axes(q, k, axes: AxisArguments, backward: bool):
@@ -230,12 +231,13 @@ def _rotate_axes(q, k, axes: AxisArguments, backward: bool):
         ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
     batch, tokens = (1, q.shape[0]) if token_major else (q.shape[0], q.shape[2])
     c, p = axes.c, axes.positions
+    pst = p.stride()
     rc = _lib.call(
         q.device, _lib.load().afa_ago_rotate_axes, q.data_ptr(), _row_strides(q, token_major), qo.data_ptr(),
         q.shape[1], *((None, None, None, 0) if k is None else
                       (k.data_ptr(), _row_strides(k, token_major), ko.data_ptr(), k.shape[1])),
         c.data_ptr(), axes.s.data_ptr(), _lib.dtype_code(c.dtype), c.shape[0], p.data_ptr(),
-        _lib.longs(p.stride(0), 0 if p.ndim == 2 else p.stride(1), p.stride(-1)), p.dtype == torch.int64,
+        _lib.longs(pst[0], 0 if len(pst) == 2 else pst[1], pst[-1]), p.dtype == torch.int64,
         axes.sections, p.shape[0], token_major, batch, tokens, q.shape[-1], backward, _lib.dtype_code(q.dtype))
     _lib.check(rc, "afa_ago_rotate_axes")
     return qo, ko
@@ -253,8 +255,13 @@ class _RotateAxes(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, gq, gk=None):
-        g = _RotateAxes.apply(gq, gk, *ctx.saved_tensors, ctx.sections, not ctx.turn_back)
-        return (*((g, None) if gk is None else g), None, None, None, None, None)
+        c, s, positions = ctx.saved_tensors
+        if torch.is_grad_enabled():  # a gradient of the gradient may follow
+            g = _RotateAxes.apply(gq, gk, c, s, positions, ctx.sections, not ctx.turn_back)
+            g = (g, None) if gk is None else g
+        else:
+            g = _rotate_axes(gq, gk, AxisArguments(c, s, positions, ctx.sections), not ctx.turn_back)
+        return (*g, None, None, None, None, None)
 
 
 def apply_ago_rotations_axes(q, k, rotary_params, positions, sections):

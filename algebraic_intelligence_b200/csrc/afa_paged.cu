@@ -469,6 +469,8 @@ extern "C" int afa_paged(const void* q, const long long* q_strides, const void* 
     snprintf(msg, sizeof(msg), "afa_paged needs a workspace of %zu bytes (got %zu)", need, workspace_bytes);
     return invalid(msg);
   }
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+    return invalid("afa_paged: the workspace must start on a 16-byte boundary");
   PagedArgs a{};
   a.q = q;
   a.k = k_cache;
@@ -487,6 +489,11 @@ extern "C" int afa_paged(const void* q, const long long* q_strides, const void* 
   a.v_sp = v_strides[0];
   a.v_sh = v_strides[1];
   a.v_sr = v_strides[2];
+  // The stride of an axis of one element says nothing: any that fits TMA does.
+  if (tokens == 1) a.q_st = 8;
+  if (q_heads == 1) a.q_sh = 8;
+  if (num_pages == 1) a.k_sp = a.v_sp = 8;
+  if (kv_heads == 1) a.k_sh = a.v_sh = 8;
   a.table_ld = table_stride;
   a.anc_ld = ancestors_stride;
   a.words = ancestor_words;

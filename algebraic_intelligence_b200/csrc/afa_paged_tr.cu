@@ -9,18 +9,21 @@
 // the octic map work on NT (16, 32 or 64) rows and not on the 128 that a row
 // tile of the other kernel has: a thread owns one key and maps NT scores, and
 // every warp has the same share whatever the number of rows. What is left is
-// the cache's bytes. With so little to map, each weight is computed in the form
-// that is exact in the negative tail (octic_exact2).
+// the cache's bytes. That leaves room for exactness: a weight enters the second
+// product as two bf16 numbers, p = hi + lo within 2^-17 (NT more columns of
+// P^T; the two halves of O^T meet in the epilogue), so that rows of few keys,
+// where the roundings of single weights do not average out, are as exact as
+// long ones.
 //
 //   warp 8      TMA: K and V tiles through a ring, in the order they are used;
 //               Q double buffered, so the next unit's loads never wait.
 //   warp 9      every tcgen05.mma, and the clearing of V rows behind a request's
 //               last token (see afa_paged_tc.cu).
 //   warps 0-7   two groups of four warps take tiles in turn: scores from TMEM,
-//               P^T to shared memory as bf16 ([key][row], 128-byte swizzle: the
-//               layout V has), row sums in registers. One group maps while the
-//               tensor core works on the other's tile.
-// TMEM columns: S^T of group g at [NT g, NT g + NT), O^T at [128, 128 + NT).
+//               P^T to shared memory as bf16 ([key][row: hi, then lo], 128-byte
+//               swizzle: the layout V has), row sums in registers. One group maps
+//               while the tensor core works on the other's tile.
+// TMEM columns: S^T of group g at [NT g, NT g + NT), O^T at [128, 128 + 2 NT).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -43,11 +46,11 @@ struct TrCfg {
   static constexpr int TILE_BYTES = KSUB * SUB_BYTES;
   static constexpr int QSUB_BYTES = NT * 128;
   static constexpr int Q_BYTES = KSUB * QSUB_BYTES;
-  static constexpr int P_BYTES = 128 * 128;
+  static constexpr int P_BYTES = (2 * NT + 63) / 64 * SUB_BYTES;  // 128 keys x 64-row blocks
   static constexpr int Q_OFF = 0;
   static constexpr int P_OFF = 2 * Q_BYTES;
   static constexpr int KV_OFF = P_OFF + 2 * P_BYTES;
-  static constexpr int NSLOT = HD == 128 ? 5 : 8;
+  static constexpr int NSLOT = HD == 128 ? (NT == 64 ? 4 : 5) : (NT == 64 ? 7 : 8);
   static constexpr int BAR_OFF = KV_OFF + NSLOT * TILE_BYTES;
   static constexpr int NBAR = 4 + 2 * NSLOT + 2 + 2 + 1 + 1;
   static constexpr int TMEM_OFF = BAR_OFF + NBAR * 8;
@@ -188,7 +191,7 @@ __global__ void __launch_bounds__(320, 1)
   } else if (warp == C::kMmaWarp) {
     // ------------------------------------------------------------------ MMA
     constexpr uint32_t idesc_s = idesc_bf16_f32(128, NT, false);
-    constexpr uint32_t idesc_o = idesc_bf16_f32(HD, NT, true) | (1u << 15);  // A = V^T: its M (head_dim) is contiguous
+    constexpr uint32_t idesc_o = idesc_bf16_f32(HD, 2 * NT, true) | (1u << 15);  // A = V^T: its M (head_dim) is contiguous
     const uint64_t q_desc = sw128_desc(smem_u32(smem + C::Q_OFF), 16, 1024);
     const uint64_t k_desc = sw128_desc(smem_u32(smem + C::KV_OFF), 16, 1024);
     const uint64_t v_desc = sw128_desc(smem_u32(smem + C::KV_OFF), C::SUB_BYTES, 1024);
@@ -266,6 +269,12 @@ __global__ void __launch_bounds__(320, 1)
     const float2 sc = make_float2(a.scale, a.scale);
     const int krow = sub * 32 + lane;  // this thread's key of a tile
     const uint32_t p_row = smem_u32(smem + C::P_OFF + g * C::P_BYTES + krow * 128);
+    // Rows [r, r + 8) of this thread's key: 16-byte chunk j of key row k lies at
+    // (j ^ (k % 8)) * 16 of the row's 128 bytes in its 64-row block.
+    auto put = [&](int r, const uint32_t (&v)[4]) {
+      const int j = (r >> 3) & 7;
+      st_shared_v4(p_row + (r >> 6) * C::SUB_BYTES + ((j ^ (krow & 7)) << 4), make_uint4(v[0], v[1], v[2], v[3]));
+    };
     int scnt = 0, oc = 0;
     bool ok = true;
     auto sync_map = [] { asm volatile("bar.sync 1, %0;" ::"r"(C::kMapWarps * 32) : "memory"); };
@@ -322,7 +331,7 @@ __global__ void __launch_bounds__(320, 1)
           const unsigned word = static_cast<unsigned>(seen >> c0);
 #pragma unroll
           for (int c = 0; c < W; c += 8) {
-            uint32_t pk[4];
+            uint32_t hi[4], lo[4];
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
               const float2 s = __fmul2_rn(make_float2(__uint_as_float(sv[c + e]), __uint_as_float(sv[c + e + 1])), sc);
@@ -331,11 +340,12 @@ __global__ void __launch_bounds__(320, 1)
               w.y = (word >> (c + e + 1)) & 1u ? w.y : 0.f;
               sum[c0 + c + e] += w.x;
               sum[c0 + c + e + 1] += w.y;
-              pk[e >> 1] = pack_bf16x2(w.x, w.y);
+              const uint32_t h = pack_bf16x2(w.x, w.y);
+              hi[e >> 1] = h;
+              lo[e >> 1] = pack_bf16x2(w.x - __uint_as_float(h << 16), w.y - __uint_as_float(h & 0xFFFF0000u));
             }
-            // 16-byte chunk j of key row k lies at (j ^ (k % 8)) * 16.
-            const int j = (c0 + c) >> 3;
-            st_shared_v4(p_row + ((j ^ (krow & 7)) << 4), make_uint4(pk[0], pk[1], pk[2], pk[3]));
+            put(c0 + c, hi);
+            put(NT + c0 + c, lo);
           }
         }
         fence_proxy_async_shared();  // P is read by the tensor core
@@ -381,8 +391,12 @@ __global__ void __launch_bounds__(320, 1)
           uint32_t ov[8];
           __syncwarp();
           if (o_here) {
+            uint32_t ol[8];
             tmem_ld8(tmem + C::O_COL + lane_off + c, ov);
+            tmem_ld8(tmem + C::O_COL + NT + lane_off + c, ol);
             tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) + __uint_as_float(ol[e]));
           } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) ov[e] = 0u;

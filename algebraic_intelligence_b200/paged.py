@@ -59,44 +59,44 @@ def _ints(name, t, shape):
 
 def _one_device(*tensors):
     """The CUDA device that all tensors live on."""
-    dev = None
+    index = tensors[0].get_device()  # -1: the host
     for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError("the paged operators need CUDA tensors")
-        if dev is not None and t.device != dev:
-            raise ValueError(f"tensors on different devices: {dev} and {t.device}")
-        dev = t.device
-    return dev
+        if t is not None and (index < 0 or t.get_device() != index):
+            if not t.is_cuda or index < 0:
+                raise ValueError("the paged operators need CUDA tensors")
+            raise ValueError(f"tensors on different devices: {tensors[0].device} and {t.device}")
+    return tensors[0].device
 
 
 def _no_gradient(what, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError(f"{what} has no gradient: call it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{what} has no gradient: call it under torch.no_grad()")
 
 
 def _caches(k_cache, v_cache, ndims=(4,)):
     """Checks a pair of caches; returns (pages, kv_heads, page_size, dim)."""
     if not isinstance(k_cache, torch.Tensor) or not isinstance(v_cache, torch.Tensor):
         raise TypeError("the caches must be tensors")
-    if k_cache.ndim not in ndims or tuple(k_cache.shape) != tuple(v_cache.shape):
+    shape = k_cache.shape
+    if len(shape) not in ndims or shape != v_cache.shape:
         raise ValueError("k_cache and v_cache must have the same (pages, kv_heads, page_size, dim) shape, got "
                          f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
     if not k_cache.is_floating_point():
         raise TypeError("expected a floating point array")
     if k_cache.dtype != v_cache.dtype:
         raise TypeError("k_cache and v_cache must share a dtype")
-    pages, heads, page_size, dim = k_cache.shape[-4:]
+    pages, heads, page_size, dim = shape[-4:]
     _check_page_size(page_size)
-    if k_cache.stride(-1) != 1 or v_cache.stride(-1) != 1:
+    if k_cache.stride()[-1] != 1 or v_cache.stride()[-1] != 1:
         raise ValueError("a cache row's channels must be contiguous")
     return pages, heads, page_size, dim
 
 
 def _rows(t):
     """A tensor whose last axis is contiguous."""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    return t if t.is_contiguous() or t.stride()[-1] == 1 else t.contiguous()
 
 
 def paged_plan(block_table, page_counts, seq_lens, new_lens, free_pages, free_count, page_size: int, max_tokens: int,
@@ -181,19 +181,20 @@ def paged_append(k, v, k_cache, v_cache, slots, q=None, rotary_params=None, posi
     transposed).
     """
     pages, heads, page_size, dim = _caches(k_cache, v_cache)
-    if k.ndim != 3 or tuple(k.shape) != tuple(v.shape) or tuple(k.shape[1:]) != (heads, dim):
+    if k.ndim != 3 or k.shape != v.shape or k.shape[1:] != (heads, dim):
         raise ValueError(f"k and v must have shape (tokens, {heads}, {dim}), got {tuple(k.shape)} and "
                          f"{tuple(v.shape)}")
     tokens = k.shape[0]
     if q is not None and (q.ndim != 3 or q.shape[0] != tokens or q.shape[2] != dim or q.shape[1] == 0):
         raise ValueError(f"q must have shape ({tokens}, heads, {dim}), got {tuple(q.shape)}")
-    if any(t is not None and t.dtype != k_cache.dtype for t in (k, v, q)):
+    dtype = k_cache.dtype
+    if k.dtype != dtype or v.dtype != dtype or (q is not None and q.dtype != dtype):
         raise TypeError("k, v, q and the caches must share a dtype")
     if k_cache.dtype == torch.float16:
         raise TypeError("float16 is not supported; use bfloat16 or float32")
     if not isinstance(slots, torch.Tensor) or slots.dtype not in (torch.int64, torch.int32):
         raise TypeError("slots must be an int64 tensor")
-    if tuple(slots.shape) != (tokens,):
+    if slots.shape != (tokens,):
         raise ValueError(f"slots must have shape ({tokens},), got {tuple(slots.shape)}")
     if dim % 2 != 0:
         raise ValueError(f"Feature dimension must be even, got {dim}")
@@ -204,22 +205,24 @@ def paged_append(k, v, k_cache, v_cache, slots, q=None, rotary_params=None, posi
     axes = axis_arguments(rotary_params, positions, sections, dim, (tokens,), dev) if rotary_params is not None \
         else None
     k, v = _rows(k), _rows(v)
-    slots = slots.to(torch.int64).contiguous()
+    if slots.dtype != torch.int64:
+        slots = slots.to(torch.int64)
+    slots = slots.contiguous()
     out = None
     if q is not None:
         q = _rows(q)
         out = torch.empty((tokens, q.shape[1], dim), dtype=q.dtype, device=dev)
     if axes is not None:
-        p = axes.positions
-        pos = (axes.c.data_ptr(), axes.s.data_ptr(), _lib.dtype_code(axes.c.dtype), axes.c.shape[0], p.data_ptr(),
-               _lib.longs(p.stride(0), p.stride(1)), int(p.dtype == torch.int64), axes.sections, p.shape[0])
+        c, p = axes.c, axes.positions
+        pos = (c.data_ptr(), axes.s.data_ptr(), _lib.dtype_code(c.dtype), c.shape[0], p.data_ptr(),
+               _lib.longs(*p.stride()), p.dtype == torch.int64, axes.sections, p.shape[0])
     else:
         pos = (None, None, 0, 0, None, None, 0, None, 0)
     rc = _lib.call(
-        dev, _lib.load().afa_paged_append, k.data_ptr(), _lib.longs(k.stride(0), k.stride(1)), v.data_ptr(), _lib.longs(v.stride(0), v.stride(1)),
+        dev, _lib.load().afa_paged_append, k.data_ptr(), _lib.longs(*k.stride()[:2]), v.data_ptr(), _lib.longs(*v.stride()[:2]),
         k_cache.data_ptr(), _lib.longs(*k_cache.stride()[:3]), v_cache.data_ptr(), _lib.longs(*v_cache.stride()[:3]),
         slots.data_ptr(), None if q is None else q.data_ptr(),
-        None if q is None else _lib.longs(q.stride(0), q.stride(1)), None if out is None else out.data_ptr(),
+        None if q is None else _lib.longs(*q.stride()[:2]), None if out is None else out.data_ptr(),
         0 if q is None else q.shape[1], *pos, tokens, heads, dim, pages, page_size,
         _lib.dtype_code(k_cache.dtype))
     _lib.check(rc, "afa_paged_append")
@@ -283,7 +286,7 @@ def afa_paged(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, ancestors=N
             raise ValueError(f"ancestors must have shape ({tokens}, words), got {tuple(ancestors.shape)}")
         words = ancestors.shape[1]
         ancestors = _rows(ancestors)
-    if out is not None and (tuple(out.shape) != tuple(q.shape) or out.dtype != q.dtype or not out.is_contiguous()):
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous()):
         raise ValueError("out must be a contiguous tensor of q's shape and dtype")
     _no_gradient("afa_paged", q, k_cache, v_cache)
     dev = _one_device(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, ancestors, out, workspace)
@@ -298,13 +301,15 @@ def afa_paged(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, ancestors=N
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
     elif not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < need:
         raise ValueError(f"workspace must be a contiguous tensor of at least {need} bytes")
+    elif workspace.data_ptr() % 16:
+        raise ValueError("workspace must start on a 16-byte boundary")
     rc = _lib.call(
-        dev, lib.afa_paged, q.data_ptr(), _lib.longs(q.stride(0), q.stride(1)), k_cache.data_ptr(), v_cache.data_ptr(),
+        dev, lib.afa_paged, q.data_ptr(), _lib.longs(*q.stride()[:2]), k_cache.data_ptr(), v_cache.data_ptr(),
         _lib.longs(*k_cache.stride()[:3]), _lib.longs(*v_cache.stride()[:3]), out.data_ptr(),
-        None if den is None else den.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+        None if den is None else den.data_ptr(), block_table.data_ptr(), block_table.stride()[0],
         seq_lens.data_ptr(), cu_tokens.data_ptr(), ancestors.data_ptr() if words else None,
         ancestors.stride(0) if words else 0, words, b, tokens, heads, kv_heads, dim, cols, page_size, pages, code,
-        float(sink_omega), workspace.data_ptr(), workspace.numel() * workspace.element_size())
+        float(sink_omega), workspace.data_ptr(), need)
     _lib.check(rc, "afa_paged")
     return (out, den) if return_denominator else out
 

@@ -331,7 +331,8 @@ AFA_API int afa_decode_noalloc(const void* q, const void* k_cache, const void* v
  *                 not written. Cached rows of a request must be finite; what
  *                 lies behind its last token does not matter.
  *                 AFA_F32, AFA_BF16, AFA_F64; D at most 256.
- *   workspace     afa_paged_workspace_bytes bytes, overwritten by each call;
+ *   workspace     afa_paged_workspace_bytes bytes on a 16-byte boundary,
+ *                 overwritten by each call;
  *                 calls that overlap need one each.
  *
  * afa_paged_commit  After a tree was verified: cache row base_lens[b] + i
