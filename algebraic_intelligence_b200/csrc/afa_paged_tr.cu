@@ -15,14 +15,16 @@
 // where the roundings of single weights do not average out, are as exact as
 // long ones.
 //
-//   warp 8      TMA: K and V tiles through a ring, in the order they are used;
+//   warp 16     TMA: K and V tiles through a ring, in the order they are used;
 //               Q double buffered, so the next unit's loads never wait.
-//   warp 9      every tcgen05.mma, and the clearing of V rows behind a request's
+//   warp 17     every tcgen05.mma, and the clearing of V rows behind a request's
 //               last token (see afa_paged_tc.cu).
-//   warps 0-7   two groups of four warps take tiles in turn: scores from TMEM,
+//   warps 0-15  two groups of eight warps take tiles in turn: scores from TMEM,
 //               P^T to shared memory as bf16 ([key][row: hi, then lo], 128-byte
 //               swizzle: the layout V has), row sums in registers. One group maps
-//               while the tensor core works on the other's tile.
+//               while the tensor core works on the other's tile; within a group
+//               four warps cover the keys of each half of the rows. (With four
+//               warps a group, 64 rows took 2.3 us a tile: one warp's chain.)
 // TMEM columns: S^T of group g at [NT g, NT g + NT), O^T at [128, 128 + 2 NT).
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -37,10 +39,11 @@ namespace {
 
 template <int HD, int NT>
 struct TrCfg {
-  static constexpr int kMapWarps = 8;
-  static constexpr int kTmaWarp = 8;
-  static constexpr int kMmaWarp = 9;
-  static constexpr int kThreads = 10 * 32;
+  static constexpr int kMapWarps = 16;
+  static constexpr int kTmaWarp = 16;
+  static constexpr int kMmaWarp = 17;
+  static constexpr int kThreads = 18 * 32;
+  static constexpr int NH = NT / 2;  // rows of a warp
   static constexpr int KSUB = HD / 64;
   static constexpr int SUB_BYTES = 128 * 128;
   static constexpr int TILE_BYTES = KSUB * SUB_BYTES;
@@ -54,11 +57,11 @@ struct TrCfg {
   static constexpr int BAR_OFF = KV_OFF + NSLOT * TILE_BYTES;
   static constexpr int NBAR = 4 + 2 * NSLOT + 2 + 2 + 1 + 1;
   static constexpr int TMEM_OFF = BAR_OFF + NBAR * 8;
-  // fp32 row sums [warp][row], then the totals [row]: in group 0's P, which no
+  // fp32 row sums [group, lane quarter][row], then the totals [row]: in group 0's P, which no
   // product reads any more when they are written.
   static constexpr int RED_OFF = P_OFF;
   static constexpr int SHARE_OFF = TMEM_OFF + 16;
-  static_assert((kMapWarps + 1) * NT * 4 <= P_BYTES, "row sums fit in P");
+  static_assert((8 + 1) * NT * 4 <= P_BYTES, "row sums fit in P");
   static constexpr int SMEM_BYTES = SHARE_OFF + (kThreads / 32 + 4) * 8 + 1024;
   static_assert(Q_BYTES % 1024 == 0 && SMEM_BYTES <= 227 * 1024, "shared memory per CTA");
   static constexpr uint32_t TMEM_COLS = 256;
@@ -71,23 +74,66 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
                : "r"(taddr));
 }
 
-// Sums of 16 values over the warp's lanes: lane l returns value l / 2's.
-__device__ __forceinline__ float reduce16(float (&v)[16], int lane) {
+// Sums of 8 values over the warp's lanes: lane l returns value l / 4's.
+__device__ __forceinline__ float reduce8(const float* v, int lane) {
+  float x[8];
 #pragma unroll
-  for (int m = 8; m >= 1; m >>= 1) {
-    const bool hi = (lane & (2 * m)) != 0;
+  for (int i = 0; i < 8; ++i) x[i] = v[i];
+#pragma unroll
+  for (int m = 4; m >= 1; m >>= 1) {
+    const bool hi = (lane & (4 * m)) != 0;
 #pragma unroll
     for (int i = 0; i < m; ++i) {
-      const float send = hi ? v[i] : v[i + m];
-      const float keep = hi ? v[i + m] : v[i];
-      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, 2 * m);
+      const float send = hi ? x[i] : x[i + m];
+      const float keep = hi ? x[i + m] : x[i];
+      x[i] = keep + __shfl_xor_sync(0xffffffffu, send, 4 * m);
     }
   }
-  return v[0] + __shfl_xor_sync(0xffffffffu, v[0], 1);
+  x[0] += __shfl_xor_sync(0xffffffffu, x[0], 2);
+  return x[0] + __shfl_xor_sync(0xffffffffu, x[0], 1);
+}
+
+// Below this score a chunk of weights is computed in the form that is exact in
+// the negative tail; above it octic_fast2 is within 2.5e-6 s^2 <= 4e-5 of a
+// weight, and one special-function operation cheaper.
+constexpr float kTrTail = -4.0f;
+
+// Weights of 8 rows for one key, as bf16 pairs hi and lo with p = hi + lo, and
+// their sums. Bit e of `seen`: row e sees the key.
+template <bool MASK>
+__device__ __forceinline__ void map8(const uint32_t* sv, float scale, unsigned seen, float* sum, uint32_t (&hi)[4],
+                                     uint32_t (&lo)[4]) {
+  const float2 sc = make_float2(scale, scale);
+  float2 s[4], w[4];
+  float least = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    s[e] = __fmul2_rn(make_float2(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), sc);
+    least = fminf(least, fminf(s[e].x, s[e].y));
+  }
+  if (__any_sync(0xffffffffu, least < kTrTail)) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = octic_exact2(s[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = octic_fast2(s[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (MASK) {
+      w[e].x = seen & (1u << (2 * e)) ? w[e].x : 0.f;
+      w[e].y = seen & (2u << (2 * e)) ? w[e].y : 0.f;
+    }
+    sum[2 * e] += w[e].x;
+    sum[2 * e + 1] += w[e].y;
+    const uint32_t h = pack_bf16x2(w[e].x, w[e].y);
+    hi[e] = h;
+    lo[e] = pack_bf16x2(w[e].x - __uint_as_float(h << 16), w[e].y - __uint_as_float(h & 0xFFFF0000u));
+  }
 }
 
 template <int HD, int NT>
-__global__ void __launch_bounds__(320, 1)
+__global__ void __launch_bounds__(576, 1)
     afa_paged_tr_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                         const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PagedArgs a) {
   using C = TrCfg<HD, NT>;
@@ -112,7 +158,7 @@ __global__ void __launch_bounds__(320, 1)
       mbar_init(q_full + i, 1);
       mbar_init(q_empty + i, 1);
       mbar_init(s_full + i, 1);
-      mbar_init(p_full + i, 4);  // one elected arrive per warp of the group
+      mbar_init(p_full + i, 8);  // one elected arrive per warp of the group
     }
     for (int s = 0; s < C::NSLOT; ++s) {
       mbar_init(kv_full + s, 1);
@@ -263,10 +309,11 @@ __global__ void __launch_bounds__(320, 1)
     __syncwarp();
   } else {
     // --------------------------------------------------- octic map + epilogue
-    const int g = warp >> 2;    // group: tiles g, g + 2, ... of a piece
-    const int sub = warp & 3;   // TMEM lane quarter
+    const int g = warp >> 3;           // group: tiles g, g + 2, ... of a piece
+    const int half = (warp >> 2) & 1;  // its half of the rows
+    const int sub = warp & 3;          // TMEM lane quarter
+    constexpr int NH = C::NH;
     const uint32_t lane_off = static_cast<uint32_t>(sub * 32) << 16;
-    const float2 sc = make_float2(a.scale, a.scale);
     const int krow = sub * 32 + lane;  // this thread's key of a tile
     const uint32_t p_row = smem_u32(smem + C::P_OFF + g * C::P_BYTES + krow * 128);
     // Rows [r, r + 8) of this thread's key: 16-byte chunk j of key row k lies at
@@ -287,9 +334,10 @@ __global__ void __launch_bounds__(320, 1)
       const int rows = left < a.unit_rows ? static_cast<int>(left) : a.unit_rows;
       const int tok_u = p.u * (a.unit_rows / a.G);  // first new token of the unit
       const int prefix = p.r.len - p.r.n;
-      float sum[NT];
+      const bool mine = half * NH < rows;  // some row of this half exists
+      float sum[NH];
 #pragma unroll
-      for (int i = 0; i < NT; ++i) sum[i] = 0.f;
+      for (int i = 0; i < NH; ++i) sum[i] = 0.f;
       for (int i = g; i < n && ok; i += 2) {
         const int key = (p.t0 + i) * kPagedTile + krow;
         bool in = key < p.r.len;
@@ -319,33 +367,27 @@ __global__ void __launch_bounds__(320, 1)
         if (!ok) break;
         tc_fence_after();
         __syncwarp();
-        constexpr int W = NT < 32 ? NT : 32;  // columns per TMEM load
-#pragma unroll
-        for (int c0 = 0; c0 < NT; c0 += W) {
-          uint32_t sv[W];
-          if constexpr (W == 32)
-            tmem_ld32(tmem + g * NT + lane_off + c0, sv);
+        if (mine) {
+          const uint32_t s_tm = tmem + g * NT + lane_off + half * NH;
+          uint32_t sv[NH];
+          if constexpr (NH == 32)
+            tmem_ld32(s_tm, sv);
+          else if constexpr (NH == 16)
+            tmem_ld16(s_tm, sv);
           else
-            tmem_ld16(tmem + g * NT + lane_off + c0, sv);
+            tmem_ld8(s_tm, sv);
           tmem_ld_wait();
-          const unsigned word = static_cast<unsigned>(seen >> c0);
+          const unsigned word = static_cast<unsigned>(seen >> (half * NH));
+          const bool all_seen = __all_sync(0xffffffffu, seen == ~0ull);
 #pragma unroll
-          for (int c = 0; c < W; c += 8) {
+          for (int c = 0; c < NH; c += 8) {
             uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-              const float2 s = __fmul2_rn(make_float2(__uint_as_float(sv[c + e]), __uint_as_float(sv[c + e + 1])), sc);
-              float2 w = octic_exact2(s);
-              w.x = (word >> (c + e)) & 1u ? w.x : 0.f;
-              w.y = (word >> (c + e + 1)) & 1u ? w.y : 0.f;
-              sum[c0 + c + e] += w.x;
-              sum[c0 + c + e + 1] += w.y;
-              const uint32_t h = pack_bf16x2(w.x, w.y);
-              hi[e >> 1] = h;
-              lo[e >> 1] = pack_bf16x2(w.x - __uint_as_float(h << 16), w.y - __uint_as_float(h & 0xFFFF0000u));
-            }
-            put(c0 + c, hi);
-            put(NT + c0 + c, lo);
+            if (all_seen)
+              map8<false>(sv + c, a.scale, 0u, sum + c, hi, lo);
+            else
+              map8<true>(sv + c, a.scale, word >> c, sum + c, hi, lo);
+            put(half * NH + c, hi);
+            put(NT + half * NH + c, lo);
           }
         }
         fence_proxy_async_shared();  // P is read by the tensor core
@@ -357,21 +399,18 @@ __global__ void __launch_bounds__(320, 1)
         ok = ok && __all_sync(0xffffffffu, mbar_wait(o_full, oc & 1, a.status, kDevTimeoutEpilogue));
         ++oc;
       }
-      // Row sums over the lanes, then over the eight warps in a fixed order.
+      // Row sums over the lanes, then over groups and lane quarters in a fixed order.
 #pragma unroll
-      for (int c = 0; c < NT; c += 16) {
-        float v[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = sum[c + i];
-        const float s = reduce16(v, lane);
-        if ((lane & 1) == 0) red[warp * NT + c + (lane >> 1)] = s;
+      for (int c = 0; c < NH; c += 8) {
+        const float s = reduce8(sum + c, lane);
+        if ((lane & 3) == 0) red[(g * 4 + sub) * NT + half * NH + c + (lane >> 2)] = s;
       }
       sync_map();
       if (threadIdx.x < NT) {
         float t = 0.f;
 #pragma unroll
-        for (int w = 0; w < C::kMapWarps; ++w) t += red[w * NT + threadIdx.x];
-        red[C::kMapWarps * NT + threadIdx.x] = t;
+        for (int w = 0; w < 8; ++w) t += red[w * NT + threadIdx.x];
+        red[8 * NT + threadIdx.x] = t;
       }
       sync_map();
       tc_fence_after();
@@ -380,14 +419,14 @@ __global__ void __launch_bounds__(320, 1)
       // accumulator uses 16 lanes of every quarter.
       const bool chan = HD == 128 || lane < 16;
       const int d = HD == 128 ? krow : sub * 16 + (lane & 15);
-      const float* tot = red + C::kMapWarps * NT;
+      const float* tot = red + 8 * NT;
       float* frag = static_cast<float*>(a.frag) + (2LL * blockIdx.x + paged_frag_slot(p)) * a.frag_rows * (HD + 1);
       __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out);
-      // The groups share the rows: 8 at a time, alternately.
+      // The four sets of warps that cover the lanes share the rows, 8 at a time.
       int tok = tok_u, head = 0;  // of row c, kept up without a division
 #pragma unroll 1
       for (int c = 0; c < NT && c < rows; c += 8) {
-        if (((c >> 3) & 1) == g) {
+        if (((c >> 3) & 3) == warp >> 2) {
           uint32_t ov[8];
           __syncwarp();
           if (o_here) {
