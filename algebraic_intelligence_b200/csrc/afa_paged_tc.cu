@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(576, 1)
   uint64_t* drain = o_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::TMEM_OFF);
   float* red = reinterpret_cast<float*>(smem + C::RED_OFF);
-  const int warp = threadIdx.x >> 5;
+  const int warp = uniform(threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   const int tile_tok = 128 / a.G;  // tokens per query tile
   const int tile_rows = tile_tok * a.G;
@@ -250,129 +250,120 @@ __global__ void __launch_bounds__(576, 1)
     const uint64_t q_desc = sw128_desc(smem_u32(smem + C::Q_OFF), 16, 1024);
     const uint64_t k_desc = sw128_desc(smem_u32(smem + C::KV_OFF), 16, 1024);
     const uint64_t v_desc = sw128_desc(smem_u32(smem + C::KV_OFF), C::SUB_BYTES, 1024);
-    // One lane issues; the branch keeps the other lanes out.
+    const uint32_t lead = lane == 0;
     auto issue_s = [&](int st, int q, int slot) {
-      const uint64_t kb = desc_add(k_desc, slot * C::TILE_BYTES);
+      const uint64_t kb = desc_add(k_desc, slot * C::TILE_BYTES), qd = desc_add(q_desc, q * C::TILE_BYTES);
 #pragma unroll
       for (int kk = 0; kk < HD / 16; ++kk) {
         const uint32_t off = (kk >> 2) * C::SUB_BYTES + (kk & 3) * 32;
-        umma_ss(tmem + C::s_col(st), desc_add(q_desc, q * C::TILE_BYTES + off), desc_add(kb, off), idesc_s,
-                kk > 0 ? 1u : 0u);
+        umma_ss_lead(lead, tmem + C::s_col(st), desc_add(qd, off), desc_add(kb, off), idesc_s, kk > 0 ? 1u : 0u);
       }
     };
     auto issue_o = [&](int st, int slot, bool acc) {
       const uint64_t vb = desc_add(v_desc, slot * C::TILE_BYTES);
 #pragma unroll
       for (int kk = 0; kk < kPagedTile / 16; ++kk)
-        umma_ts(tmem + C::o_col(st), tmem + C::s_col(st) + C::p_col(kk), desc_add(vb, kk * 2048), idesc_o,
-                (acc || kk > 0) ? 1u : 0u);
+        umma_ts_lead(lead, tmem + C::o_col(st), tmem + C::s_col(st) + C::p_col(kk), desc_add(vb, kk * 2048), idesc_o,
+                     (acc || kk > 0) ? 1u : 0u);
     };
-    int qn = 0, u = 0, pc[2] = {0, 0};
+    int qn = 0, pc0 = 0, pc1 = 0;
+    RingPos<C::NSLOT> kv;
     bool ok = true;
-    auto wait_kv = [&](int x) {
-      return mbar_wait(kv_full + x % C::NSLOT, (x / C::NSLOT) & 1, a.status, kDevTimeoutMma);
+    auto wait_kv = [&](const RingPos<C::NSLOT>& x) {
+      return __all_sync(0xffffffffu, mbar_wait(kv_full + x.slot, x.phase, a.status, kDevTimeoutMma));
+    };
+    auto wait_p = [&](int st) {
+      const int phase = st ? pc1++ : pc0++;
+      return __all_sync(0xffffffffu, mbar_wait(p_full + st, phase & 1, a.status, kDevTimeoutMma));
     };
     while (ok && walk.next(a, p)) {
       const PgPiece g = pg_piece(a, p, tile_rows);
-      const int n = g.n;
+      const int n = uniform(g.n), n0 = uniform(g.n0), t0 = uniform(p.t0), len = uniform(p.r.len);
       if (n == 0) continue;
       auto clear_tail = [&](int i, int slot) {
-        clear_v_tail<C::KSUB>(smem + C::KV_OFF + slot * C::TILE_BYTES, p.r.len - (p.t0 + i) * kPagedTile, a.page_shift,
+        clear_v_tail<C::KSUB>(smem + C::KV_OFF + slot * C::TILE_BYTES, len - (t0 + i) * kPagedTile, a.page_shift,
                               lane);
       };
       if (!(ok = __all_sync(0xffffffffu, mbar_wait(q_full, qn & 1, a.status, kDevTimeoutMma)))) break;
       ++qn;
-      if (g.split) {
-        for (int i = 0; ok && i < min(2, n); ++i, ++u) {
-          if (!(ok = __all_sync(0xffffffffu, wait_kv(u)))) break;
+      if (uniform(g.split)) {
+        for (int i = 0; ok && i < min(2, n); ++i) {
+          if (!(ok = wait_kv(kv))) break;
           tc_fence_after();
-          if (lane == 0) {
-            issue_s(i, 0, u % C::NSLOT);
-            umma_commit(s_full + i);
-            umma_commit(kv_empty + u % C::NSLOT);
-            if (i + 1 == n) umma_commit(q_empty);
-          }
+          issue_s(i, 0, kv.slot);
+          umma_commit_lead(lead, s_full + i);
+          umma_commit_lead(lead, kv_empty + kv.slot);
+          if (i + 1 == n) umma_commit_lead(lead, q_empty);
+          kv.step();
         }
         for (int i = 0; ok && i < n; ++i) {
-          const int st = i & 1;
-          const int sv = u % C::NSLOT;
-          if (!(ok = __all_sync(0xffffffffu, wait_kv(u)))) break;
-          clear_tail(i, sv);
+          const int st = i & 1, sv = kv.slot;
           const bool more = i + 2 < n;
-          const int sk = (u + 1) % C::NSLOT;
-          if (more && !(ok = __all_sync(0xffffffffu, wait_kv(u + 1)))) break;
-          if (!(ok = __all_sync(0xffffffffu, mbar_wait(p_full + st, pc[st] & 1, a.status, kDevTimeoutMma)))) break;
-          ++pc[st];
+          if (!(ok = wait_kv(kv))) break;
+          clear_tail(i, sv);
+          kv.step();
+          if (more && !(ok = wait_kv(kv))) break;
+          if (!(ok = wait_p(st))) break;
           tc_fence_after();
-          if (lane == 0) {
-            issue_o(st, sv, i >= 2);
-            umma_commit(kv_empty + sv);
-            if (!more) umma_commit(o_full + st);
-            if (more) {
-              issue_s(st, 0, sk);
-              umma_commit(s_full + st);
-              umma_commit(kv_empty + sk);
-              if (i + 3 == n) umma_commit(q_empty);
-            }
+          issue_o(st, sv, i >= 2);
+          umma_commit_lead(lead, kv_empty + sv);
+          if (!more) umma_commit_lead(lead, o_full + st);
+          if (more) {
+            issue_s(st, 0, kv.slot);
+            umma_commit_lead(lead, s_full + st);
+            umma_commit_lead(lead, kv_empty + kv.slot);
+            if (i + 3 == n) umma_commit_lead(lead, q_empty);
+            kv.step();
           }
-          u += more ? 2 : 1;
         }
       } else {
-        if (!(ok = __all_sync(0xffffffffu, wait_kv(u)))) break;
+        if (!(ok = wait_kv(kv))) break;
         tc_fence_after();
-        if (lane == 0) {
-          if (g.n0 > 0) {
-            issue_s(0, 0, u % C::NSLOT);
-            umma_commit(s_full + 0);
-          }
-          issue_s(1, 1, u % C::NSLOT);
-          umma_commit(s_full + 1);
-          umma_commit(kv_empty + u % C::NSLOT);
-          if (n == 1) umma_commit(q_empty);
+        if (n0 > 0) {
+          issue_s(0, 0, kv.slot);
+          umma_commit_lead(lead, s_full + 0);
         }
-        ++u;
+        issue_s(1, 1, kv.slot);
+        umma_commit_lead(lead, s_full + 1);
+        umma_commit_lead(lead, kv_empty + kv.slot);
+        if (n == 1) umma_commit_lead(lead, q_empty);
+        kv.step();
         for (int i = 0; ok && i < n; ++i) {
-          const int sv = u % C::NSLOT, sk = (u + 1) % C::NSLOT;
+          const int sv = kv.slot;
           const bool more = i + 1 < n;
-          if (!(ok = __all_sync(0xffffffffu, wait_kv(u)))) break;
+          if (!(ok = wait_kv(kv))) break;
           clear_tail(i, sv);
-          if (more && !(ok = __all_sync(0xffffffffu, wait_kv(u + 1)))) break;
-          if (i < g.n0) {
-            if (!(ok = __all_sync(0xffffffffu, mbar_wait(p_full + 0, pc[0] & 1, a.status, kDevTimeoutMma)))) break;
-            ++pc[0];
+          kv.step();
+          const int sk = kv.slot;
+          if (more && !(ok = wait_kv(kv))) break;
+          if (i < n0) {
+            if (!(ok = wait_p(0))) break;
             tc_fence_after();
-            if (lane == 0) {
-              issue_o(0, sv, i > 0);
-              if (i + 1 == g.n0) umma_commit(o_full + 0);
-              if (i + 1 < g.n0) {
-                issue_s(0, 0, sk);
-                umma_commit(s_full + 0);
-              }
+            issue_o(0, sv, i > 0);
+            if (i + 1 == n0) umma_commit_lead(lead, o_full + 0);
+            if (i + 1 < n0) {
+              issue_s(0, 0, sk);
+              umma_commit_lead(lead, s_full + 0);
             }
           }
-          if (!(ok = __all_sync(0xffffffffu, mbar_wait(p_full + 1, pc[1] & 1, a.status, kDevTimeoutMma)))) break;
-          ++pc[1];
+          if (!(ok = wait_p(1))) break;
           tc_fence_after();
-          if (lane == 0) {
-            issue_o(1, sv, i > 0);
-            umma_commit(kv_empty + sv);
-            if (!more) umma_commit(o_full + 1);
-            if (more) {
-              issue_s(1, 1, sk);
-              umma_commit(s_full + 1);
-              umma_commit(kv_empty + sk);
-              if (i + 2 == n) umma_commit(q_empty);
-            }
+          issue_o(1, sv, i > 0);
+          umma_commit_lead(lead, kv_empty + sv);
+          if (!more) umma_commit_lead(lead, o_full + 1);
+          if (more) {
+            issue_s(1, 1, sk);
+            umma_commit_lead(lead, s_full + 1);
+            umma_commit_lead(lead, kv_empty + sk);
+            if (i + 2 == n) umma_commit_lead(lead, q_empty);
+            kv.step();
           }
-          u += more ? 2 : 1;
         }
       }
     }
     // Every MMA issued must finish before TMEM is released.
-    if (lane == 0) {
-      umma_commit(drain);
-      (void)mbar_wait(drain, 0, nullptr, 0);
-    }
+    umma_commit_lead(lead, drain);
+    (void)mbar_wait(drain, 0, nullptr, 0);
     __syncwarp();
   } else {
     // --------------------------------------------------- octic map + epilogue

@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(576, 1)
   uint64_t* drain = o_full + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::TMEM_OFF);
   float* red = reinterpret_cast<float*>(smem + C::RED_OFF);
-  const int warp = threadIdx.x >> 5;
+  const int warp = uniform(threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -242,70 +242,67 @@ __global__ void __launch_bounds__(576, 1)
     const uint64_t k_desc = sw128_desc(smem_u32(smem + C::KV_OFF), 16, 1024);
     const uint64_t v_desc = sw128_desc(smem_u32(smem + C::KV_OFF), C::SUB_BYTES, 1024);
     const uint64_t p_desc = sw128_desc(smem_u32(smem + C::P_OFF), C::SUB_BYTES, 1024);
+    const uint32_t lead = lane == 0;
     auto issue_s = [&](int g, int qb, int slot) {
       const uint64_t kb = desc_add(k_desc, slot * C::TILE_BYTES), qd = desc_add(q_desc, qb * C::Q_BYTES);
 #pragma unroll
       for (int kk = 0; kk < HD / 16; ++kk)
-        umma_ss(tmem + g * NT, desc_add(kb, (kk >> 2) * C::SUB_BYTES + (kk & 3) * 32),
-                desc_add(qd, (kk >> 2) * C::QSUB_BYTES + (kk & 3) * 32), idesc_s, kk > 0 ? 1u : 0u);
+        umma_ss_lead(lead, tmem + g * NT, desc_add(kb, (kk >> 2) * C::SUB_BYTES + (kk & 3) * 32),
+                     desc_add(qd, (kk >> 2) * C::QSUB_BYTES + (kk & 3) * 32), idesc_s, kk > 0 ? 1u : 0u);
     };
     auto issue_o = [&](int g, int slot, bool acc) {
       const uint64_t vb = desc_add(v_desc, slot * C::TILE_BYTES), pd = desc_add(p_desc, g * C::P_BYTES);
 #pragma unroll
       for (int kk = 0; kk < kPagedTile / 16; ++kk)
-        umma_ss(tmem + C::O_COL, desc_add(vb, kk * 2048), desc_add(pd, kk * 2048), idesc_o, (acc || kk > 0) ? 1u : 0u);
+        umma_ss_lead(lead, tmem + C::O_COL, desc_add(vb, kk * 2048), desc_add(pd, kk * 2048), idesc_o,
+                     (acc || kk > 0) ? 1u : 0u);
     };
-    int qn = 0, u = 0, pc0 = 0, pc1 = 0;
+    int qn = 0, pc0 = 0, pc1 = 0;
+    RingPos<C::NSLOT> kv;
     bool ok = true;
-    auto wait_kv = [&](int x) {
-      return __all_sync(0xffffffffu,
-                        mbar_wait(kv_full + x % C::NSLOT, (x / C::NSLOT) & 1, a.status, kDevTimeoutMma));
+    auto wait_kv = [&](const RingPos<C::NSLOT>& x) {
+      return __all_sync(0xffffffffu, mbar_wait(kv_full + x.slot, x.phase, a.status, kDevTimeoutMma));
     };
     while (ok && walk.next(a, p)) {
-      const int n = p.tiles > 0 ? p.t1 - p.t0 : 0;
+      const int t0 = uniform(p.t0), n = uniform(p.tiles > 0 ? p.t1 : p.t0) - t0, len = uniform(p.r.len);
       if (n == 0) continue;
       const int qb = qn & 1;
       if (!(ok = __all_sync(0xffffffffu, mbar_wait(q_full + qb, (qn >> 1) & 1, a.status, kDevTimeoutMma)))) break;
       ++qn;
-      for (int i = 0; ok && i < min(2, n); ++i, ++u) {
-        if (!(ok = wait_kv(u))) break;
+      for (int i = 0; ok && i < min(2, n); ++i) {
+        if (!(ok = wait_kv(kv))) break;
         tc_fence_after();
-        if (lane == 0) {
-          issue_s(i, qb, u % C::NSLOT);
-          umma_commit(s_full + i);
-          umma_commit(kv_empty + u % C::NSLOT);
-          if (i + 1 == n) umma_commit(q_empty + qb);
-        }
+        issue_s(i, qb, kv.slot);
+        umma_commit_lead(lead, s_full + i);
+        umma_commit_lead(lead, kv_empty + kv.slot);
+        if (i + 1 == n) umma_commit_lead(lead, q_empty + qb);
+        kv.step();
       }
       for (int i = 0; ok && i < n; ++i) {
-        const int g = i & 1, sv = u % C::NSLOT, sk = (u + 1) % C::NSLOT;
+        const int g = i & 1, sv = kv.slot;
         const bool more = i + 2 < n;
-        if (!(ok = wait_kv(u))) break;
-        clear_v_tail<C::KSUB>(smem + C::KV_OFF + sv * C::TILE_BYTES, p.r.len - (p.t0 + i) * kPagedTile, a.page_shift,
-                              lane);
-        if (more && !(ok = wait_kv(u + 1))) break;
+        if (!(ok = wait_kv(kv))) break;
+        clear_v_tail<C::KSUB>(smem + C::KV_OFF + sv * C::TILE_BYTES, len - (t0 + i) * kPagedTile, a.page_shift, lane);
+        kv.step();
+        if (more && !(ok = wait_kv(kv))) break;
         const int phase = g ? pc1++ : pc0++;
         if (!(ok = __all_sync(0xffffffffu, mbar_wait(p_full + g, phase & 1, a.status, kDevTimeoutMma)))) break;
         tc_fence_after();
-        if (lane == 0) {
-          issue_o(g, sv, i > 0);
-          umma_commit(kv_empty + sv);
-          if (i + 1 == n) umma_commit(o_full);
-          if (more) {
-            issue_s(g, qb, sk);
-            umma_commit(s_full + g);
-            umma_commit(kv_empty + sk);
-            if (i + 3 == n) umma_commit(q_empty + qb);
-          }
+        issue_o(g, sv, i > 0);
+        umma_commit_lead(lead, kv_empty + sv);
+        if (i + 1 == n) umma_commit_lead(lead, o_full);
+        if (more) {
+          issue_s(g, qb, kv.slot);
+          umma_commit_lead(lead, s_full + g);
+          umma_commit_lead(lead, kv_empty + kv.slot);
+          if (i + 3 == n) umma_commit_lead(lead, q_empty + qb);
+          kv.step();
         }
-        u += more ? 2 : 1;
       }
     }
     // Every MMA issued must finish before TMEM is released.
-    if (lane == 0) {
-      umma_commit(drain);
-      (void)mbar_wait(drain, 0, nullptr, 0);
-    }
+    umma_commit_lead(lead, drain);
+    (void)mbar_wait(drain, 0, nullptr, 0);
     __syncwarp();
   } else {
     // --------------------------------------------------- octic map + epilogue
