@@ -250,20 +250,19 @@ __global__ void __launch_bounds__(576, 1)
     const uint64_t q_desc = sw128_desc(smem_u32(smem + C::Q_OFF), 16, 1024);
     const uint64_t k_desc = sw128_desc(smem_u32(smem + C::KV_OFF), 16, 1024);
     const uint64_t v_desc = sw128_desc(smem_u32(smem + C::KV_OFF), C::SUB_BYTES, 1024);
-    const uint32_t lead = lane == 0;
     auto issue_s = [&](int st, int q, int slot) {
       const uint64_t kb = desc_add(k_desc, slot * C::TILE_BYTES), qd = desc_add(q_desc, q * C::TILE_BYTES);
 #pragma unroll
       for (int kk = 0; kk < HD / 16; ++kk) {
         const uint32_t off = (kk >> 2) * C::SUB_BYTES + (kk & 3) * 32;
-        umma_ss_lead(lead, tmem + C::s_col(st), desc_add(qd, off), desc_add(kb, off), idesc_s, kk > 0 ? 1u : 0u);
+        umma_ss(tmem + C::s_col(st), desc_add(qd, off), desc_add(kb, off), idesc_s, kk > 0 ? 1u : 0u);
       }
     };
     auto issue_o = [&](int st, int slot, bool acc) {
       const uint64_t vb = desc_add(v_desc, slot * C::TILE_BYTES);
 #pragma unroll
       for (int kk = 0; kk < kPagedTile / 16; ++kk)
-        umma_ts_lead(lead, tmem + C::o_col(st), tmem + C::s_col(st) + C::p_col(kk), desc_add(vb, kk * 2048), idesc_o,
+        umma_ts(tmem + C::o_col(st), tmem + C::s_col(st) + C::p_col(kk), desc_add(vb, kk * 2048), idesc_o,
                      (acc || kk > 0) ? 1u : 0u);
     };
     int qn = 0, pc0 = 0, pc1 = 0;
@@ -290,10 +289,12 @@ __global__ void __launch_bounds__(576, 1)
         for (int i = 0; ok && i < min(2, n); ++i) {
           if (!(ok = wait_kv(kv))) break;
           tc_fence_after();
-          issue_s(i, 0, kv.slot);
-          umma_commit_lead(lead, s_full + i);
-          umma_commit_lead(lead, kv_empty + kv.slot);
-          if (i + 1 == n) umma_commit_lead(lead, q_empty);
+          if (elect_one()) {
+            issue_s(i, 0, kv.slot);
+            umma_commit(s_full + i);
+            umma_commit(kv_empty + kv.slot);
+            if (i + 1 == n) umma_commit(q_empty);
+          }
           kv.step();
         }
         for (int i = 0; ok && i < n; ++i) {
@@ -305,28 +306,33 @@ __global__ void __launch_bounds__(576, 1)
           if (more && !(ok = wait_kv(kv))) break;
           if (!(ok = wait_p(st))) break;
           tc_fence_after();
-          issue_o(st, sv, i >= 2);
-          umma_commit_lead(lead, kv_empty + sv);
-          if (!more) umma_commit_lead(lead, o_full + st);
-          if (more) {
-            issue_s(st, 0, kv.slot);
-            umma_commit_lead(lead, s_full + st);
-            umma_commit_lead(lead, kv_empty + kv.slot);
-            if (i + 3 == n) umma_commit_lead(lead, q_empty);
-            kv.step();
+          if (elect_one()) {
+            issue_o(st, sv, i >= 2);
+            umma_commit(kv_empty + sv);
+            if (more) {
+              issue_s(st, 0, kv.slot);
+              umma_commit(s_full + st);
+              umma_commit(kv_empty + kv.slot);
+              if (i + 3 == n) umma_commit(q_empty);
+            } else {
+              umma_commit(o_full + st);
+            }
           }
+          if (more) kv.step();
         }
       } else {
         if (!(ok = wait_kv(kv))) break;
         tc_fence_after();
-        if (n0 > 0) {
-          issue_s(0, 0, kv.slot);
-          umma_commit_lead(lead, s_full + 0);
+        if (elect_one()) {
+          if (n0 > 0) {
+            issue_s(0, 0, kv.slot);
+            umma_commit(s_full + 0);
+          }
+          issue_s(1, 1, kv.slot);
+          umma_commit(s_full + 1);
+          umma_commit(kv_empty + kv.slot);
+          if (n == 1) umma_commit(q_empty);
         }
-        issue_s(1, 1, kv.slot);
-        umma_commit_lead(lead, s_full + 1);
-        umma_commit_lead(lead, kv_empty + kv.slot);
-        if (n == 1) umma_commit_lead(lead, q_empty);
         kv.step();
         for (int i = 0; ok && i < n; ++i) {
           const int sv = kv.slot;
@@ -339,30 +345,36 @@ __global__ void __launch_bounds__(576, 1)
           if (i < n0) {
             if (!(ok = wait_p(0))) break;
             tc_fence_after();
-            issue_o(0, sv, i > 0);
-            if (i + 1 == n0) umma_commit_lead(lead, o_full + 0);
-            if (i + 1 < n0) {
-              issue_s(0, 0, sk);
-              umma_commit_lead(lead, s_full + 0);
+            if (elect_one()) {
+              issue_o(0, sv, i > 0);
+              if (i + 1 < n0) {
+                issue_s(0, 0, sk);
+                umma_commit(s_full + 0);
+              } else {
+                umma_commit(o_full + 0);
+              }
             }
           }
           if (!(ok = wait_p(1))) break;
           tc_fence_after();
-          issue_o(1, sv, i > 0);
-          umma_commit_lead(lead, kv_empty + sv);
-          if (!more) umma_commit_lead(lead, o_full + 1);
-          if (more) {
-            issue_s(1, 1, sk);
-            umma_commit_lead(lead, s_full + 1);
-            umma_commit_lead(lead, kv_empty + sk);
-            if (i + 2 == n) umma_commit_lead(lead, q_empty);
-            kv.step();
+          if (elect_one()) {
+            issue_o(1, sv, i > 0);
+            umma_commit(kv_empty + sv);
+            if (more) {
+              issue_s(1, 1, sk);
+              umma_commit(s_full + 1);
+              umma_commit(kv_empty + sk);
+              if (i + 2 == n) umma_commit(q_empty);
+            } else {
+              umma_commit(o_full + 1);
+            }
           }
+          if (more) kv.step();
         }
       }
     }
     // Every MMA issued must finish before TMEM is released.
-    umma_commit_lead(lead, drain);
+    if (elect_one()) umma_commit(drain);
     (void)mbar_wait(drain, 0, nullptr, 0);
     __syncwarp();
   } else {

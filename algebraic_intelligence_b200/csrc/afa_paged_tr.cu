@@ -242,19 +242,18 @@ __global__ void __launch_bounds__(576, 1)
     const uint64_t k_desc = sw128_desc(smem_u32(smem + C::KV_OFF), 16, 1024);
     const uint64_t v_desc = sw128_desc(smem_u32(smem + C::KV_OFF), C::SUB_BYTES, 1024);
     const uint64_t p_desc = sw128_desc(smem_u32(smem + C::P_OFF), C::SUB_BYTES, 1024);
-    const uint32_t lead = lane == 0;
     auto issue_s = [&](int g, int qb, int slot) {
       const uint64_t kb = desc_add(k_desc, slot * C::TILE_BYTES), qd = desc_add(q_desc, qb * C::Q_BYTES);
 #pragma unroll
       for (int kk = 0; kk < HD / 16; ++kk)
-        umma_ss_lead(lead, tmem + g * NT, desc_add(kb, (kk >> 2) * C::SUB_BYTES + (kk & 3) * 32),
+        umma_ss(tmem + g * NT, desc_add(kb, (kk >> 2) * C::SUB_BYTES + (kk & 3) * 32),
                      desc_add(qd, (kk >> 2) * C::QSUB_BYTES + (kk & 3) * 32), idesc_s, kk > 0 ? 1u : 0u);
     };
     auto issue_o = [&](int g, int slot, bool acc) {
       const uint64_t vb = desc_add(v_desc, slot * C::TILE_BYTES), pd = desc_add(p_desc, g * C::P_BYTES);
 #pragma unroll
       for (int kk = 0; kk < kPagedTile / 16; ++kk)
-        umma_ss_lead(lead, tmem + C::O_COL, desc_add(vb, kk * 2048), desc_add(pd, kk * 2048), idesc_o,
+        umma_ss(tmem + C::O_COL, desc_add(vb, kk * 2048), desc_add(pd, kk * 2048), idesc_o,
                      (acc || kk > 0) ? 1u : 0u);
     };
     int qn = 0, pc0 = 0, pc1 = 0;
@@ -272,10 +271,12 @@ __global__ void __launch_bounds__(576, 1)
       for (int i = 0; ok && i < min(2, n); ++i) {
         if (!(ok = wait_kv(kv))) break;
         tc_fence_after();
-        issue_s(i, qb, kv.slot);
-        umma_commit_lead(lead, s_full + i);
-        umma_commit_lead(lead, kv_empty + kv.slot);
-        if (i + 1 == n) umma_commit_lead(lead, q_empty + qb);
+        if (elect_one()) {
+          issue_s(i, qb, kv.slot);
+          umma_commit(s_full + i);
+          umma_commit(kv_empty + kv.slot);
+          if (i + 1 == n) umma_commit(q_empty + qb);
+        }
         kv.step();
       }
       for (int i = 0; ok && i < n; ++i) {
@@ -288,20 +289,22 @@ __global__ void __launch_bounds__(576, 1)
         const int phase = g ? pc1++ : pc0++;
         if (!(ok = __all_sync(0xffffffffu, mbar_wait(p_full + g, phase & 1, a.status, kDevTimeoutMma)))) break;
         tc_fence_after();
-        issue_o(g, sv, i > 0);
-        umma_commit_lead(lead, kv_empty + sv);
-        if (i + 1 == n) umma_commit_lead(lead, o_full);
-        if (more) {
-          issue_s(g, qb, kv.slot);
-          umma_commit_lead(lead, s_full + g);
-          umma_commit_lead(lead, kv_empty + kv.slot);
-          if (i + 3 == n) umma_commit_lead(lead, q_empty + qb);
-          kv.step();
+        if (elect_one()) {
+          issue_o(g, sv, i > 0);
+          umma_commit(kv_empty + sv);
+          if (i + 1 == n) umma_commit(o_full);
+          if (more) {
+            issue_s(g, qb, kv.slot);
+            umma_commit(s_full + g);
+            umma_commit(kv_empty + kv.slot);
+            if (i + 3 == n) umma_commit(q_empty + qb);
+          }
         }
+        if (more) kv.step();
       }
     }
     // Every MMA issued must finish before TMEM is released.
-    umma_commit_lead(lead, drain);
+    if (elect_one()) umma_commit(drain);
     (void)mbar_wait(drain, 0, nullptr, 0);
     __syncwarp();
   } else {
