@@ -53,7 +53,7 @@ struct PgCfg {
   static constexpr int Q_OFF = 0;
   static constexpr int KV_OFF = 2 * TILE_BYTES;
   static constexpr int BAR_OFF = KV_OFF + NSLOT * TILE_BYTES;
-  static constexpr int NBAR = 2 + 2 * NSLOT + 2 + 2 + 2 + 1;
+  static constexpr int NBAR = 4 + 2 * NSLOT + 2 + 2 + 2 + 1;
   static constexpr int TMEM_OFF = BAR_OFF + NBAR * 8;
   static constexpr int RED_OFF = TMEM_OFF + 8;               // fp32 row sums [stream][row]
   static constexpr int SHARE_OFF = RED_OFF + 2 * 128 * 4;    // scratch of paged_share
@@ -132,6 +132,25 @@ __device__ __forceinline__ PgPiece pg_piece(const PagedArgs& a, const PagedPiece
   return g;
 }
 
+// The two query buffers: a pair takes both, a split piece the one used less, so
+// that a split piece's queries load while the piece before still runs. Loader
+// and MMA warp keep the same count.
+struct QBuffers {
+  int uses[2] = {0, 0};
+  int first = 0, last = 0;  // of this piece
+  __device__ __forceinline__ void next(bool split) {
+    first = split && uses[1] < uses[0] ? 1 : 0;
+    last = split ? first : 1;
+  }
+  __device__ __forceinline__ uint32_t phase(int i) const { return (i ? uses[1] : uses[0]) & 1; }
+  __device__ __forceinline__ void take(int i) {
+    if (i)
+      ++uses[1];
+    else
+      ++uses[0];
+  }
+};
+
 template <int HD>
 __global__ void __launch_bounds__(576, 1)
     afa_paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -141,8 +160,8 @@ __global__ void __launch_bounds__(576, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
   uint64_t* q_full = bars;
-  uint64_t* q_empty = bars + 1;
-  uint64_t* kv_full = bars + 2;
+  uint64_t* q_empty = bars + 2;
+  uint64_t* kv_full = bars + 4;
   uint64_t* kv_empty = kv_full + C::NSLOT;
   uint64_t* s_full = kv_empty + C::NSLOT;
   uint64_t* p_full = s_full + 2;
@@ -156,8 +175,10 @@ __global__ void __launch_bounds__(576, 1)
   const int tile_rows = tile_tok * a.G;
 
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(q_full + i, 1);
+      mbar_init(q_empty + i, 1);
+    }
     for (int s = 0; s < C::NSLOT; ++s) {
       mbar_init(kv_full + s, 1);
       mbar_init(kv_empty + s, 1);
@@ -191,23 +212,26 @@ __global__ void __launch_bounds__(576, 1)
   if (warp == C::kTmaWarp) {
     // ------------------------------------------------------------------ TMA
     KvPages pages(a);
-    int u = 0, qn = 0;
+    int u = 0;
+    QBuffers qb;
     bool ok = true;
     while (ok && walk.next(a, p)) {
       if (lane == 0) paged_meta_piece(a.meta, p);
       const PgPiece g = pg_piece(a, p, tile_rows);
       if (g.n == 0) continue;
-      // The previous piece's last S = Q K^T must be done with the Q tiles.
-      if (qn > 0 && !(ok = mbar_wait(q_empty, (qn - 1) & 1, a.status, kDevTimeoutProducer))) break;
-      if (lane == 0) {
-        const int tiles = g.split ? 1 : 2;
-        mbar_arrive_expect_tx(q_full, tiles * C::KSUB * tile_rows * 128);
-        for (int i = 0; i < tiles; ++i)
+      qb.next(g.split);
+      for (int i = qb.first; ok && i <= qb.last; ++i) {
+        // The last S = Q K^T of the piece that held this buffer must be done.
+        ok = __all_sync(0xffffffffu, mbar_wait(q_empty + i, qb.phase(i) ^ 1, a.status, kDevTimeoutProducer));
+        if (ok && lane == 0) {
+          mbar_arrive_expect_tx(q_full + i, C::KSUB * tile_rows * 128);
           for (int h = 0; h < C::KSUB; ++h)
-            tma_load_4d(smem + C::Q_OFF + (i * C::KSUB + h) * C::SUB_BYTES, &tm_q, q_full, 64 * h, 0, p.h,
-                        p.r.tok0 + (p.u * 2 + i) * tile_tok);
+            tma_load_4d(smem + C::Q_OFF + (i * C::KSUB + h) * C::SUB_BYTES, &tm_q, q_full + i, 64 * h, 0, p.h,
+                        p.r.tok0 + (p.u * 2 + i - qb.first) * tile_tok);
+        }
+        if (ok) qb.take(i);
       }
-      ++qn;
+      if (!ok) break;
       auto load = [&](int i, bool v, int page) {  // tile i of the piece
         const int slot = u % C::NSLOT;
         if (!(ok = ok && __all_sync(0xffffffffu, mbar_wait(kv_empty + slot, ((u / C::NSLOT) & 1) ^ 1, a.status,
@@ -240,7 +264,8 @@ __global__ void __launch_bounds__(576, 1)
       }
     }
     // Do not leave the CTA while loads into its shared memory are in flight.
-    if (qn > 0) (void)mbar_wait(q_full, (qn - 1) & 1, nullptr, 0);
+    for (int i = 0; i < 2; ++i)
+      if (qb.uses[i] > 0) (void)mbar_wait(q_full + i, (qb.uses[i] - 1) & 1, nullptr, 0);
     for (int x = u - C::NSLOT < 0 ? 0 : u - C::NSLOT; x < u; ++x)
       (void)mbar_wait(kv_full + (x % C::NSLOT), (x / C::NSLOT) & 1, nullptr, 0);
   } else if (warp == C::kMmaWarp) {
@@ -265,7 +290,8 @@ __global__ void __launch_bounds__(576, 1)
         umma_ts(tmem + C::o_col(st), tmem + C::s_col(st) + C::p_col(kk), desc_add(vb, kk * 2048), idesc_o,
                      (acc || kk > 0) ? 1u : 0u);
     };
-    int qn = 0, pc0 = 0, pc1 = 0;
+    int pc0 = 0, pc1 = 0;
+    QBuffers qb;
     RingPos<C::NSLOT> kv;
     bool ok = true;
     auto wait_kv = [&](const RingPos<C::NSLOT>& x) {
@@ -283,17 +309,23 @@ __global__ void __launch_bounds__(576, 1)
         clear_v_tail<C::KSUB>(smem + C::KV_OFF + slot * C::TILE_BYTES, len - (t0 + i) * kPagedTile, a.page_shift,
                               lane);
       };
-      if (!(ok = __all_sync(0xffffffffu, mbar_wait(q_full, qn & 1, a.status, kDevTimeoutMma)))) break;
-      ++qn;
-      if (uniform(g.split)) {
+      const bool split = uniform(g.split);
+      qb.next(split);
+      for (int i = qb.first; ok && i <= qb.last; ++i) {
+        ok = __all_sync(0xffffffffu, mbar_wait(q_full + i, qb.phase(i), a.status, kDevTimeoutMma));
+        qb.take(i);
+      }
+      if (!ok) break;
+      const int q0 = uniform(qb.first);
+      if (split) {
         for (int i = 0; ok && i < min(2, n); ++i) {
           if (!(ok = wait_kv(kv))) break;
           tc_fence_after();
           if (elect_one()) {
-            issue_s(i, 0, kv.slot);
+            issue_s(i, q0, kv.slot);
             umma_commit(s_full + i);
             umma_commit(kv_empty + kv.slot);
-            if (i + 1 == n) umma_commit(q_empty);
+            if (i + 1 == n) umma_commit(q_empty + q0);
           }
           kv.step();
         }
@@ -310,10 +342,10 @@ __global__ void __launch_bounds__(576, 1)
             issue_o(st, sv, i >= 2);
             umma_commit(kv_empty + sv);
             if (more) {
-              issue_s(st, 0, kv.slot);
+              issue_s(st, q0, kv.slot);
               umma_commit(s_full + st);
               umma_commit(kv_empty + kv.slot);
-              if (i + 3 == n) umma_commit(q_empty);
+              if (i + 3 == n) umma_commit(q_empty + q0);
             } else {
               umma_commit(o_full + st);
             }
@@ -331,7 +363,10 @@ __global__ void __launch_bounds__(576, 1)
           issue_s(1, 1, kv.slot);
           umma_commit(s_full + 1);
           umma_commit(kv_empty + kv.slot);
-          if (n == 1) umma_commit(q_empty);
+          if (n == 1) {
+            umma_commit(q_empty + 0);
+            umma_commit(q_empty + 1);
+          }
         }
         kv.step();
         for (int i = 0; ok && i < n; ++i) {
@@ -364,7 +399,10 @@ __global__ void __launch_bounds__(576, 1)
               issue_s(1, 1, sk);
               umma_commit(s_full + 1);
               umma_commit(kv_empty + sk);
-              if (i + 2 == n) umma_commit(q_empty);
+              if (i + 2 == n) {
+                umma_commit(q_empty + 0);
+                umma_commit(q_empty + 1);
+              }
             } else {
               umma_commit(o_full + 1);
             }
@@ -405,19 +443,19 @@ __global__ void __launch_bounds__(576, 1)
       const int nmap = g.split || st ? g.n : g.n0;
       float dsum = 0.f;
       bool tail_check = true;  // warp-uniform: some row's weights so far < kTailRowSum
+      // This lane's table entry of tile i, read a tile ahead of its use.
+      auto entry = [&](int i) {
+        const int key = (p.t0 + i) * kPagedTile + lane * ps;
+        return busy && i < nmap && lane < per_tile && key < p.r.len
+                   ? a.table[p.b * a.table_ld + (key >> a.page_shift)]
+                   : 0;
+      };
+      int next_entry = entry(first);
       for (int i = first; i < nmap && ok; i += step) {
         const int key0 = (p.t0 + i) * kPagedTile;
         // Pages of the tile that the table does not name in the cache.
-        unsigned bad = 0;
-        if (busy) {
-          bool b = false;
-          const int key = key0 + lane * ps;
-          if (lane < per_tile && key < p.r.len) {
-            const int e = a.table[p.b * a.table_ld + (key >> a.page_shift)];
-            b = e < 0 || e >= a.num_pages;
-          }
-          bad = __ballot_sync(0xffffffffu, b);
-        }
+        const unsigned bad = __ballot_sync(0xffffffffu, next_entry < 0 || next_entry >= a.num_pages);
+        next_entry = entry(i + step);
         ok = __all_sync(0xffffffffu, mbar_wait(s_full + st, sc & 1, a.status, kDevTimeoutSoftmax));
         ++sc;
         if (!ok) break;

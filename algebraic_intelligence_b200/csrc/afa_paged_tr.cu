@@ -338,13 +338,17 @@ __global__ void __launch_bounds__(576, 1)
       float sum[NH];
 #pragma unroll
       for (int i = 0; i < NH; ++i) sum[i] = 0.f;
+      // Table entry of this thread's key of tile i, read a tile ahead; -1 where
+      // there is no key.
+      auto entry = [&](int i) {
+        const int key = (p.t0 + i) * kPagedTile + krow;
+        return i < n && key < p.r.len ? a.table[p.b * a.table_ld + (key >> a.page_shift)] : -1;
+      };
+      int next_entry = entry(g);
       for (int i = g; i < n && ok; i += 2) {
         const int key = (p.t0 + i) * kPagedTile + krow;
-        bool in = key < p.r.len;
-        if (in) {
-          const int e = a.table[p.b * a.table_ld + (key >> a.page_shift)];
-          in = e >= 0 && e < a.num_pages;
-        }
+        const bool in = next_entry >= 0 && next_entry < a.num_pages;
+        next_entry = entry(i + 2);
         // Rows that see this thread's key.
         unsigned long long seen = in ? ~0ull : 0ull;
         const int at = key - prefix;
