@@ -25,7 +25,12 @@
 //               while the tensor core works on the other's tile; within a group
 //               four warps cover the keys of each half of the rows. (With four
 //               warps a group, 64 rows took 2.3 us a tile: one warp's chain.)
-// TMEM columns: S^T of group g at [NT g, NT g + NT), O^T at [128, 128 + 2 NT).
+//               A piece's output is written after the next piece's scores were
+//               mapped (O^T and the row sums are double buffered), so that no
+//               warp waits for the last P.V: in batches of short requests that
+//               wait and the barriers around it were most of the time.
+// TMEM columns: S^T of group g at [NT g, NT g + NT), O^T of every other piece at
+// [128, 128 + 2 NT) and [128 + 2 NT, 128 + 4 NT).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -51,21 +56,20 @@ struct TrCfg {
   static constexpr int Q_BYTES = KSUB * QSUB_BYTES;
   static constexpr int P_BYTES = (2 * NT + 63) / 64 * SUB_BYTES;  // 128 keys x 64-row blocks
   static constexpr int Q_OFF = 0;
-  static constexpr int P_OFF = 2 * Q_BYTES;
+  static constexpr int QBUF = NT == 64 && HD == 128 ? 1 : 2;  // query buffers: what shared memory leaves
+  static constexpr int P_OFF = QBUF * Q_BYTES;
   static constexpr int KV_OFF = P_OFF + 2 * P_BYTES;
   static constexpr int NSLOT = HD == 128 ? (NT == 64 ? 4 : 5) : (NT == 64 ? 7 : 8);
   static constexpr int BAR_OFF = KV_OFF + NSLOT * TILE_BYTES;
-  static constexpr int NBAR = 4 + 2 * NSLOT + 2 + 2 + 1 + 1;
+  static constexpr int NBAR = 4 + 2 * NSLOT + 2 + 2 + 2 + 2 + 2 + 1;
   static constexpr int TMEM_OFF = BAR_OFF + NBAR * 8;
-  // fp32 row sums [group, lane quarter][row], then the totals [row]: in group 0's P, which no
-  // product reads any more when they are written.
-  static constexpr int RED_OFF = P_OFF;
-  static constexpr int SHARE_OFF = TMEM_OFF + 16;
-  static_assert((8 + 1) * NT * 4 <= P_BYTES, "row sums fit in P");
-  static constexpr int SMEM_BYTES = SHARE_OFF + (kThreads / 32 + 4) * 8 + 1024;
+  static constexpr int RED_OFF = TMEM_OFF + 16;  // fp32 row sums [piece parity][group, lane quarter][row]
+  static constexpr int SHARE_OFF = RED_OFF;      // paged_share's scratch: before any sum is written
+  static_assert((kThreads / 32 + 4) * 8 <= 2 * 8 * NT * 4, "scratch fits in the sums");
+  static constexpr int SMEM_BYTES = RED_OFF + 2 * 8 * NT * 4 + 1024;
   static_assert(Q_BYTES % 1024 == 0 && SMEM_BYTES <= 227 * 1024, "shared memory per CTA");
-  static constexpr uint32_t TMEM_COLS = 256;
-  static constexpr uint32_t O_COL = 128;
+  static constexpr uint32_t TMEM_COLS = NT == 64 ? 512 : 256;
+  __device__ static constexpr uint32_t o_col(int parity) { return 128u + static_cast<uint32_t>(parity) * 2 * NT; }
 };
 
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
@@ -147,7 +151,9 @@ __global__ void __launch_bounds__(576, 1)
   uint64_t* s_full = kv_empty + C::NSLOT;
   uint64_t* p_full = s_full + 2;
   uint64_t* o_full = p_full + 2;
-  uint64_t* drain = o_full + 1;
+  uint64_t* o_empty = o_full + 2;   // a piece's outputs are written: its O^T and row sums may be overwritten
+  uint64_t* r_full = o_empty + 2;   // every warp's row sums are written
+  uint64_t* drain = r_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::TMEM_OFF);
   float* red = reinterpret_cast<float*>(smem + C::RED_OFF);
   const int warp = uniform(threadIdx.x >> 5);
@@ -159,12 +165,14 @@ __global__ void __launch_bounds__(576, 1)
       mbar_init(q_empty + i, 1);
       mbar_init(s_full + i, 1);
       mbar_init(p_full + i, 8);  // one elected arrive per warp of the group
+      mbar_init(o_full + i, 1);
+      mbar_init(o_empty + i, C::kMapWarps);
+      mbar_init(r_full + i, C::kMapWarps);
     }
     for (int s = 0; s < C::NSLOT; ++s) {
       mbar_init(kv_full + s, 1);
       mbar_init(kv_empty + s, 1);
     }
-    mbar_init(o_full, 1);
     mbar_init(drain, 1);
     fence_barrier_init();
     fence_proxy_async_smem();
@@ -195,8 +203,9 @@ __global__ void __launch_bounds__(576, 1)
       if (lane == 0) paged_meta_piece(a.meta, p);
       const int n = p.tiles > 0 ? p.t1 - p.t0 : 0;
       if (n == 0) continue;
-      const int qb = qn & 1;
-      if (!(ok = __all_sync(0xffffffffu, mbar_wait(q_empty + qb, ((qn >> 1) & 1) ^ 1, a.status, kDevTimeoutProducer))))
+      const int qb = qn % C::QBUF;
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(q_empty + qb, ((qn / C::QBUF) & 1) ^ 1, a.status,
+                                                   kDevTimeoutProducer))))
         break;
       if (lane == 0) {
         mbar_arrive_expect_tx(q_full + qb, C::KSUB * a.unit_rows * 128);
@@ -231,7 +240,8 @@ __global__ void __launch_bounds__(576, 1)
       }
     }
     // Do not leave the CTA while loads into its shared memory are in flight.
-    for (int x = qn - 2 < 0 ? 0 : qn - 2; x < qn; ++x) (void)mbar_wait(q_full + (x & 1), (x >> 1) & 1, nullptr, 0);
+    for (int x = qn - C::QBUF < 0 ? 0 : qn - C::QBUF; x < qn; ++x)
+      (void)mbar_wait(q_full + x % C::QBUF, (x / C::QBUF) & 1, nullptr, 0);
     for (int x = u - C::NSLOT < 0 ? 0 : u - C::NSLOT; x < u; ++x)
       (void)mbar_wait(kv_full + (x % C::NSLOT), (x / C::NSLOT) & 1, nullptr, 0);
   } else if (warp == C::kMmaWarp) {
@@ -249,14 +259,14 @@ __global__ void __launch_bounds__(576, 1)
         umma_ss(tmem + g * NT, desc_add(kb, (kk >> 2) * C::SUB_BYTES + (kk & 3) * 32),
                      desc_add(qd, (kk >> 2) * C::QSUB_BYTES + (kk & 3) * 32), idesc_s, kk > 0 ? 1u : 0u);
     };
-    auto issue_o = [&](int g, int slot, bool acc) {
+    auto issue_o = [&](int g, int par, int slot, bool acc) {
       const uint64_t vb = desc_add(v_desc, slot * C::TILE_BYTES), pd = desc_add(p_desc, g * C::P_BYTES);
 #pragma unroll
       for (int kk = 0; kk < kPagedTile / 16; ++kk)
-        umma_ss(tmem + C::O_COL, desc_add(vb, kk * 2048), desc_add(pd, kk * 2048), idesc_o,
-                     (acc || kk > 0) ? 1u : 0u);
+        umma_ss(tmem + C::o_col(par), desc_add(vb, kk * 2048), desc_add(pd, kk * 2048), idesc_o,
+                (acc || kk > 0) ? 1u : 0u);
     };
-    int qn = 0, pc0 = 0, pc1 = 0;
+    int qn = 0, pc0 = 0, pc1 = 0, piece = -1;
     RingPos<C::NSLOT> kv;
     bool ok = true;
     auto wait_kv = [&](const RingPos<C::NSLOT>& x) {
@@ -264,9 +274,10 @@ __global__ void __launch_bounds__(576, 1)
     };
     while (ok && walk.next(a, p)) {
       const int t0 = uniform(p.t0), n = uniform(p.tiles > 0 ? p.t1 : p.t0) - t0, len = uniform(p.r.len);
+      ++piece;
       if (n == 0) continue;
-      const int qb = qn & 1;
-      if (!(ok = __all_sync(0xffffffffu, mbar_wait(q_full + qb, (qn >> 1) & 1, a.status, kDevTimeoutMma)))) break;
+      const int par = piece & 1, qb = qn % C::QBUF;
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(q_full + qb, (qn / C::QBUF) & 1, a.status, kDevTimeoutMma)))) break;
       ++qn;
       for (int i = 0; ok && i < min(2, n); ++i) {
         if (!(ok = wait_kv(kv))) break;
@@ -288,11 +299,14 @@ __global__ void __launch_bounds__(576, 1)
         if (more && !(ok = wait_kv(kv))) break;
         const int phase = g ? pc1++ : pc0++;
         if (!(ok = __all_sync(0xffffffffu, mbar_wait(p_full + g, phase & 1, a.status, kDevTimeoutMma)))) break;
+        if (i == 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(o_empty + par, ((piece >> 1) & 1) ^ 1, a.status,
+                                                                kDevTimeoutMma))))
+          break;
         tc_fence_after();
         if (elect_one()) {
-          issue_o(g, sv, i > 0);
+          issue_o(g, par, sv, i > 0);
           umma_commit(kv_empty + sv);
-          if (i + 1 == n) umma_commit(o_full);
+          if (i + 1 == n) umma_commit(o_full + par);
           if (more) {
             issue_s(g, qb, kv.slot);
             umma_commit(s_full + g);
@@ -322,16 +336,75 @@ __global__ void __launch_bounds__(576, 1)
       const int j = (r >> 3) & 7;
       st_shared_v4(p_row + (r >> 6) * C::SUB_BYTES + ((j ^ (krow & 7)) << 4), make_uint4(v[0], v[1], v[2], v[3]));
     };
-    int scnt = 0, oc = 0;
+    int scnt = 0, piece = -1;
+    int oc[2] = {0, 0};  // pieces with an O^T, by parity
     bool ok = true;
-    auto sync_map = [] { asm volatile("bar.sync 1, %0;" ::"r"(C::kMapWarps * 32) : "memory"); };
-    // Every warp walks every piece and meets at the same barriers, also after
-    // a wait ran out (ok false).
+    // Outputs of a piece: O / (sum + sink), or the fragment.
+    int d_rows = 0, d_tok = 0, d_h = 0, d_kind = 0;  // of the piece to write: kind bit 0 whole, 1 later fragment, 2 has O
+    auto write_piece = [&](int par, int use) {
+      const bool whole = d_kind & 1, has_o = d_kind & 4;
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(r_full + par, use & 1, a.status, kDevTimeoutEpilogue));
+      if (has_o) {
+        const int phase = par ? oc[1]++ : oc[0]++;
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(o_full + par, phase & 1, a.status, kDevTimeoutEpilogue));
+      }
+      tc_fence_after();
+      const bool o_here = ok && has_o;
+      // Head channel of this thread's TMEM lane: with 64 channels (M = 64) the
+      // accumulator uses 16 lanes of every quarter.
+      const bool chan = HD == 128 || lane < 16;
+      const int d = HD == 128 ? krow : sub * 16 + (lane & 15);
+      const float* r = red + par * 8 * NT;
+      float* frag = static_cast<float*>(a.frag) + (2LL * blockIdx.x + ((d_kind >> 1) & 1)) * a.frag_rows * (HD + 1);
+      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out);
+      // The four sets of warps that cover the lanes share the rows, 8 at a time.
+#pragma unroll 1
+      for (int c = 8 * (warp >> 2); c < d_rows; c += 32) {
+        float total = 0.f;  // of row c + lane % 8; groups and quarters in a fixed order
+#pragma unroll
+        for (int w = 0; w < 8; ++w) total += r[w * NT + c + (lane & 7)];
+        const float denom = total + a.sink;
+        const float scale_o = whole ? (denom > 0.f ? 1.0f / denom : 0.f) : 1.f;
+        uint32_t ov[8], ol[8];
+        __syncwarp();
+        if (o_here) {
+          tmem_ld8(tmem + C::o_col(par) + lane_off + c, ov);
+          tmem_ld8(tmem + C::o_col(par) + NT + lane_off + c, ol);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) ov[e] = ol[e] = 0u;
+        }
+        const int row = c + (lane & 7), tok = row / a.G;
+        const long long my_row = static_cast<long long>(d_tok + tok) * a.Hkv * a.G +
+                                 static_cast<long long>(d_h) * a.G + (row - tok * a.G);
+        if (sub == 0 && lane < 8 && row < d_rows) {
+          if (!whole)
+            frag[static_cast<long long>(a.frag_rows) * HD + row] = total;
+          else if (a.dtot)
+            static_cast<float*>(a.dtot)[my_row] = denom;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float y = (__uint_as_float(ov[e]) + __uint_as_float(ol[e])) * __shfl_sync(0xffffffffu, scale_o, e);
+          const long long orow = __shfl_sync(0xffffffffu, my_row, e);
+          if (chan && c + e < d_rows) {
+            if (whole)
+              out[orow * HD + d] = __float2bfloat16_rn(y);
+            else
+              frag[static_cast<long long>(c + e) * HD + d] = y;
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(o_empty + par);
+    };
+    // Every warp walks every piece, also after a wait ran out (ok false).
     while (walk.next(a, p)) {
+      ++piece;
       const int n = p.tiles > 0 ? p.t1 - p.t0 : 0;
-      const long long row0 = static_cast<long long>(p.u) * a.unit_rows;
-      const long long left = static_cast<long long>(p.r.n) * a.G - row0;
-      const int rows = left < a.unit_rows ? static_cast<int>(left) : a.unit_rows;
+      const int row0 = p.u * a.unit_rows, rows = min(p.r.n * a.G - row0, a.unit_rows);
       const int tok_u = p.u * (a.unit_rows / a.G);  // first new token of the unit
       const int prefix = p.r.len - p.r.n;
       const bool mine = half * NH < rows;  // some row of this half exists
@@ -399,84 +472,24 @@ __global__ void __launch_bounds__(576, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full + g);
       }
-      if (n > 0) {
-        ok = ok && __all_sync(0xffffffffu, mbar_wait(o_full, oc & 1, a.status, kDevTimeoutEpilogue));
-        ++oc;
-      }
-      // Row sums over the lanes, then over groups and lane quarters in a fixed order.
+      // Row sums over the lanes, into this parity's buffer once the outputs of
+      // the piece before the last are written.
+      const int par = piece & 1, use = piece >> 1;
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(o_empty + par, (use & 1) ^ 1, a.status, kDevTimeoutEpilogue));
 #pragma unroll
       for (int c = 0; c < NH; c += 8) {
         const float s = reduce8(sum + c, lane);
-        if ((lane & 3) == 0) red[(g * 4 + sub) * NT + half * NH + c + (lane >> 2)] = s;
+        if ((lane & 3) == 0) red[par * 8 * NT + (g * 4 + sub) * NT + half * NH + c + (lane >> 2)] = s;
       }
-      sync_map();
-      if (threadIdx.x < NT) {
-        float t = 0.f;
-#pragma unroll
-        for (int w = 0; w < 8; ++w) t += red[w * NT + threadIdx.x];
-        red[8 * NT + threadIdx.x] = t;
-      }
-      sync_map();
-      tc_fence_after();
-      const bool whole = p.whole(), o_here = ok && n > 0;
-      // Head channel of this thread's TMEM lane: with 64 channels (M = 64) the
-      // accumulator uses 16 lanes of every quarter.
-      const bool chan = HD == 128 || lane < 16;
-      const int d = HD == 128 ? krow : sub * 16 + (lane & 15);
-      const float* tot = red + 8 * NT;
-      float* frag = static_cast<float*>(a.frag) + (2LL * blockIdx.x + paged_frag_slot(p)) * a.frag_rows * (HD + 1);
-      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out);
-      // The four sets of warps that cover the lanes share the rows, 8 at a time.
-      int tok = tok_u, head = 0;  // of row c, kept up without a division
-#pragma unroll 1
-      for (int c = 0; c < NT && c < rows; c += 8) {
-        if (((c >> 3) & 3) == warp >> 2) {
-          uint32_t ov[8];
-          __syncwarp();
-          if (o_here) {
-            uint32_t ol[8];
-            tmem_ld8(tmem + C::O_COL + lane_off + c, ov);
-            tmem_ld8(tmem + C::O_COL + NT + lane_off + c, ol);
-            tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 8; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) + __uint_as_float(ol[e]));
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) ov[e] = 0u;
-          }
-          int t = tok, hh = head;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            if (c + e < rows) {
-              const float den = tot[c + e] + a.sink;
-              const long long orow = (static_cast<long long>(p.r.tok0) + t) * a.Hkv * a.G +
-                                     static_cast<long long>(p.h) * a.G + hh;
-              if (whole) {
-                const float y = den > 0.f ? __uint_as_float(ov[e]) / den : 0.f;
-                if (chan) out[orow * HD + d] = __float2bfloat16_rn(y);
-                if (a.dtot && threadIdx.x % 128 == 0) static_cast<float*>(a.dtot)[orow] = den;
-              } else {
-                if (chan) frag[static_cast<long long>(c + e) * HD + d] = __uint_as_float(ov[e]);
-                if (threadIdx.x % 128 == 0) frag[static_cast<long long>(a.frag_rows) * HD + c + e] = tot[c + e];
-              }
-            }
-            if (++hh == a.G) {
-              hh = 0;
-              ++t;
-            }
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (++head == a.G) {
-            head = 0;
-            ++tok;
-          }
-      }
-      // O and the sums are read: the next piece's first P may be announced.
-      tc_fence_before();
-      sync_map();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(r_full + par);
+      if (piece > 0) write_piece(par ^ 1, (piece - 1) >> 1);
+      d_rows = rows;
+      d_tok = p.r.tok0 + tok_u;
+      d_h = p.h;
+      d_kind = (p.whole() ? 1 : 0) | paged_frag_slot(p) << 1 | (n > 0 ? 4 : 0);
     }
+    if (piece >= 0) write_piece(piece & 1, piece >> 1);
   }
 
   tc_fence_before();
