@@ -13,8 +13,8 @@
 //          Octic sums only add, so the two O accumulators meet in the epilogue.
 // Warps whose 32 rows are all beyond the unit's last row skip the map.
 //
-//   warp 16     TMA: lane l loads page l of a tile (K, then V, 64-column halves,
-//               128-byte swizzle). Tiles are loaded in the order the tensor core
+//   warps 16,18 TMA, K (and Q) and V: lane l loads page l of a tile (64-column
+//               halves, 128-byte swizzle). Tiles are loaded in the order the tensor core
 //               consumes them: LA K tiles first (2 split, 1 pair), then V_i,
 //               K_{i + LA}, so ring slots free up in order. Pages behind a
 //               request's last token and entries that name no page are given a
@@ -45,7 +45,8 @@ struct PgCfg {
   static constexpr int kOcticWarps = 16;
   static constexpr int kTmaWarp = 16;
   static constexpr int kMmaWarp = 17;
-  static constexpr int kThreads = 18 * 32;
+  static constexpr int kTmaVWarp = 18;
+  static constexpr int kThreads = 19 * 32;
   static constexpr int KSUB = HD / 64;
   static constexpr int SUB_BYTES = 128 * 128;  // 128 rows x 128 B
   static constexpr int TILE_BYTES = KSUB * SUB_BYTES;
@@ -152,7 +153,7 @@ struct QBuffers {
 };
 
 template <int HD>
-__global__ void __launch_bounds__(576, 1)
+__global__ void __launch_bounds__(608, 1)
     afa_paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                         const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PagedArgs a) {
   using C = PgCfg<HD>;
@@ -209,18 +210,19 @@ __global__ void __launch_bounds__(576, 1)
   const uint32_t tmem = *tmem_slot;
   PagedPiece p;
 
-  if (warp == C::kTmaWarp) {
+  if (warp == C::kTmaWarp || warp == C::kTmaVWarp) {
     // ------------------------------------------------------------------ TMA
+    const bool is_v = warp == C::kTmaVWarp;
     KvPages pages(a);
     int u = 0;
     QBuffers qb;
     bool ok = true;
     while (ok && walk.next(a, p)) {
-      if (lane == 0) paged_meta_piece(a.meta, p);
+      if (!is_v && lane == 0) paged_meta_piece(a.meta, p);
       const PgPiece g = pg_piece(a, p, tile_rows);
       if (g.n == 0) continue;
       qb.next(g.split);
-      for (int i = qb.first; ok && i <= qb.last; ++i) {
+      for (int i = qb.first; ok && !is_v && i <= qb.last; ++i) {
         // The last S = Q K^T of the piece that held this buffer must be done.
         ok = __all_sync(0xffffffffu, mbar_wait(q_empty + i, qb.phase(i) ^ 1, a.status, kDevTimeoutProducer));
         if (ok && lane == 0) {
@@ -233,15 +235,15 @@ __global__ void __launch_bounds__(576, 1)
       }
       if (!ok) break;
       auto load = [&](int i, bool v, int page) {  // tile i of the piece
-        const int slot = u % C::NSLOT;
-        if (!(ok = ok && __all_sync(0xffffffffu, mbar_wait(kv_empty + slot, ((u / C::NSLOT) & 1) ^ 1, a.status,
+        const int slot = u++ % C::NSLOT;
+        if (v != is_v) return;  // the other warp's
+        if (!(ok = ok && __all_sync(0xffffffffu, mbar_wait(kv_empty + slot, (((u - 1) / C::NSLOT) & 1) ^ 1, a.status,
                                                            kDevTimeoutProducer))))
           return;
         if (lane == 0) mbar_arrive_expect_tx(kv_full + slot, C::TILE_BYTES);
         __syncwarp();
         pages.template load<C::KSUB>(smem + C::KV_OFF + slot * C::TILE_BYTES, v ? &tm_v : &tm_k, kv_full + slot,
                                      p, i, page);
-        ++u;
       };
       // Table entries are read three tiles ahead of their loads' use, so no
       // load waits for them.

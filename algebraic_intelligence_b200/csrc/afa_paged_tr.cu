@@ -15,8 +15,10 @@
 // where the roundings of single weights do not average out, are as exact as
 // long ones.
 //
-//   warp 16     TMA: K and V tiles through a ring, in the order they are used;
-//               Q double buffered, so the next unit's loads never wait.
+//   warps 16,18 TMA: K (and Q) and V tiles through one ring, in the order they
+//               are used; Q double buffered, so the next unit's loads never wait.
+//               With pages of 16 tokens a tile of K and V is 32 copies of 65
+//               cycles each to issue, more than one warp has time for.
 //   warp 17     every tcgen05.mma, and the clearing of V rows behind a request's
 //               last token (see afa_paged_tc.cu).
 //   warps 0-15  two groups of eight warps take tiles in turn: scores from TMEM,
@@ -47,7 +49,8 @@ struct TrCfg {
   static constexpr int kMapWarps = 16;
   static constexpr int kTmaWarp = 16;
   static constexpr int kMmaWarp = 17;
-  static constexpr int kThreads = 18 * 32;
+  static constexpr int kTmaVWarp = 18;
+  static constexpr int kThreads = 19 * 32;
   static constexpr int NH = NT / 2;  // rows of a warp
   static constexpr int KSUB = HD / 64;
   static constexpr int SUB_BYTES = 128 * 128;
@@ -76,6 +79,19 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                : "r"(taddr));
+}
+
+// N columns (1, 2 or 4) of this thread's lane.
+template <int N>
+__device__ __forceinline__ void tmem_ld_few(uint32_t taddr, uint32_t (&r)[N]) {
+  if constexpr (N == 1)
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r[0]) : "r"(taddr));
+  else if constexpr (N == 2)
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(taddr));
+  else
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(taddr));
 }
 
 // Sums of 8 values over the warp's lanes: lane l returns value l / 4's.
@@ -137,7 +153,7 @@ __device__ __forceinline__ void map8(const uint32_t* sv, float scale, unsigned s
 }
 
 template <int HD, int NT>
-__global__ void __launch_bounds__(576, 1)
+__global__ void __launch_bounds__(608, 1)
     afa_paged_tr_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                         const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PagedArgs a) {
   using C = TrCfg<HD, NT>;
@@ -194,20 +210,21 @@ __global__ void __launch_bounds__(576, 1)
   const uint32_t tmem = *tmem_slot;
   PagedPiece p;
 
-  if (warp == C::kTmaWarp) {
+  if (warp == C::kTmaWarp || warp == C::kTmaVWarp) {
     // ------------------------------------------------------------------ TMA
+    const bool is_v = warp == C::kTmaVWarp;
     KvPages pages(a);
     int u = 0, qn = 0;
     bool ok = true;
     while (ok && walk.next(a, p)) {
-      if (lane == 0) paged_meta_piece(a.meta, p);
+      if (!is_v && lane == 0) paged_meta_piece(a.meta, p);
       const int n = p.tiles > 0 ? p.t1 - p.t0 : 0;
       if (n == 0) continue;
       const int qb = qn % C::QBUF;
-      if (!(ok = __all_sync(0xffffffffu, mbar_wait(q_empty + qb, ((qn / C::QBUF) & 1) ^ 1, a.status,
-                                                   kDevTimeoutProducer))))
+      if (!is_v && !(ok = __all_sync(0xffffffffu, mbar_wait(q_empty + qb, ((qn / C::QBUF) & 1) ^ 1, a.status,
+                                                            kDevTimeoutProducer))))
         break;
-      if (lane == 0) {
+      if (!is_v && lane == 0) {
         mbar_arrive_expect_tx(q_full + qb, C::KSUB * a.unit_rows * 128);
         for (int h = 0; h < C::KSUB; ++h)
           tma_load_4d(smem + C::Q_OFF + qb * C::Q_BYTES + h * C::QSUB_BYTES, &tm_q, q_full + qb, 64 * h, 0, p.h,
@@ -215,15 +232,15 @@ __global__ void __launch_bounds__(576, 1)
       }
       ++qn;
       auto load = [&](int i, bool v, int page) {
-        const int slot = u % C::NSLOT;
-        if (!(ok = ok && __all_sync(0xffffffffu, mbar_wait(kv_empty + slot, ((u / C::NSLOT) & 1) ^ 1, a.status,
+        const int slot = u++ % C::NSLOT;
+        if (v != is_v) return;  // the other warp's
+        if (!(ok = ok && __all_sync(0xffffffffu, mbar_wait(kv_empty + slot, (((u - 1) / C::NSLOT) & 1) ^ 1, a.status,
                                                            kDevTimeoutProducer))))
           return;
         if (lane == 0) mbar_arrive_expect_tx(kv_full + slot, C::TILE_BYTES);
         __syncwarp();
         pages.template load<C::KSUB>(smem + C::KV_OFF + slot * C::TILE_BYTES, v ? &tm_v : &tm_k, kv_full + slot,
                                      p, i, page);
-        ++u;
       };
       int page[4];
 #pragma unroll
@@ -357,37 +374,40 @@ __global__ void __launch_bounds__(576, 1)
       const float* r = red + par * 8 * NT;
       float* frag = static_cast<float*>(a.frag) + (2LL * blockIdx.x + ((d_kind >> 1) & 1)) * a.frag_rows * (HD + 1);
       __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out);
-      // The four sets of warps that cover the lanes share the rows, 8 at a time.
+      // The four sets of warps that cover the lanes share the rows, a few at a
+      // time so that all have some of a single token's.
+      constexpr int CH = NT / 16;
 #pragma unroll 1
-      for (int c = 8 * (warp >> 2); c < d_rows; c += 32) {
-        float total = 0.f;  // of row c + lane % 8; groups and quarters in a fixed order
+      for (int c = CH * (warp >> 2); c < d_rows; c += 4 * CH) {
+        float total = 0.f;  // of row c + lane % CH; groups and quarters in a fixed order
 #pragma unroll
-        for (int w = 0; w < 8; ++w) total += r[w * NT + c + (lane & 7)];
+        for (int w = 0; w < 8; ++w) total += r[w * NT + c + lane % CH];
         const float denom = total + a.sink;
-        const float scale_o = whole ? (denom > 0.f ? 1.0f / denom : 0.f) : 1.f;
-        uint32_t ov[8], ol[8];
+        const float scale_o = whole ? (denom > 0.f ? __frcp_rn(denom) : 0.f) : 1.f;
+        uint32_t ov[CH], ol[CH];
         __syncwarp();
         if (o_here) {
-          tmem_ld8(tmem + C::o_col(par) + lane_off + c, ov);
-          tmem_ld8(tmem + C::o_col(par) + NT + lane_off + c, ol);
+          tmem_ld_few<CH>(tmem + C::o_col(par) + lane_off + c, ov);
+          tmem_ld_few<CH>(tmem + C::o_col(par) + NT + lane_off + c, ol);
           tmem_ld_wait();
         } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) ov[e] = ol[e] = 0u;
+          for (int e = 0; e < CH; ++e) ov[e] = ol[e] = 0u;
         }
-        const int row = c + (lane & 7), tok = row / a.G;
+        const int row = c + lane % CH, tok = row / a.G;
         const long long my_row = static_cast<long long>(d_tok + tok) * a.Hkv * a.G +
                                  static_cast<long long>(d_h) * a.G + (row - tok * a.G);
-        if (sub == 0 && lane < 8 && row < d_rows) {
+        if (sub == 0 && lane < CH && row < d_rows) {
           if (!whole)
             frag[static_cast<long long>(a.frag_rows) * HD + row] = total;
           else if (a.dtot)
             static_cast<float*>(a.dtot)[my_row] = denom;
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float y = (__uint_as_float(ov[e]) + __uint_as_float(ol[e])) * __shfl_sync(0xffffffffu, scale_o, e);
-          const long long orow = __shfl_sync(0xffffffffu, my_row, e);
+        for (int e = 0; e < CH; ++e) {
+          const float y = (__uint_as_float(ov[e]) + __uint_as_float(ol[e])) *
+                          (CH > 1 ? __shfl_sync(0xffffffffu, scale_o, e) : scale_o);
+          const long long orow = CH > 1 ? __shfl_sync(0xffffffffu, my_row, e) : my_row;
           if (chan && c + e < d_rows) {
             if (whole)
               out[orow * HD + d] = __float2bfloat16_rn(y);
@@ -401,7 +421,15 @@ __global__ void __launch_bounds__(576, 1)
       if (lane == 0) mbar_arrive(o_empty + par);
     };
     // Every warp walks every piece, also after a wait ran out (ok false).
-    while (walk.next(a, p)) {
+    // Table entry of this thread's key of tile i, read a tile (or a piece) ahead
+    // of its use; -1 where there is no key.
+    auto entry = [&](int i) {
+      const int key = (p.t0 + i) * kPagedTile + krow;
+      return p.t0 + i < p.t1 && key < p.r.len ? a.table[p.b * a.table_ld + (key >> a.page_shift)] : -1;
+    };
+    bool have = walk.next(a, p);
+    int next_entry = have ? entry(g) : -1;
+    while (have) {
       ++piece;
       const int n = p.tiles > 0 ? p.t1 - p.t0 : 0;
       const int row0 = p.u * a.unit_rows, rows = min(p.r.n * a.G - row0, a.unit_rows);
@@ -411,13 +439,6 @@ __global__ void __launch_bounds__(576, 1)
       float sum[NH];
 #pragma unroll
       for (int i = 0; i < NH; ++i) sum[i] = 0.f;
-      // Table entry of this thread's key of tile i, read a tile ahead; -1 where
-      // there is no key.
-      auto entry = [&](int i) {
-        const int key = (p.t0 + i) * kPagedTile + krow;
-        return i < n && key < p.r.len ? a.table[p.b * a.table_ld + (key >> a.page_shift)] : -1;
-      };
-      int next_entry = entry(g);
       for (int i = g; i < n && ok; i += 2) {
         const int key = (p.t0 + i) * kPagedTile + krow;
         const bool in = next_entry >= 0 && next_entry < a.num_pages;
@@ -483,11 +504,24 @@ __global__ void __launch_bounds__(576, 1)
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(r_full + par);
+      const int tok = p.r.tok0 + tok_u, head = p.h;
+      const int kind = (p.whole() ? 1 : 0) | paged_frag_slot(p) << 1 | (n > 0 ? 4 : 0);
+      // The next piece's first table entry is under way while the outputs are
+      // written (with 64 rows there are no registers to hold it).
+      constexpr bool kAhead = NT < 64;
+      if (kAhead) {
+        have = walk.next(a, p);
+        next_entry = have ? entry(g) : -1;
+      }
       if (piece > 0) write_piece(par ^ 1, (piece - 1) >> 1);
       d_rows = rows;
-      d_tok = p.r.tok0 + tok_u;
-      d_h = p.h;
-      d_kind = (p.whole() ? 1 : 0) | paged_frag_slot(p) << 1 | (n > 0 ? 4 : 0);
+      d_tok = tok;
+      d_h = head;
+      d_kind = kind;
+      if (!kAhead) {
+        have = walk.next(a, p);
+        next_entry = have ? entry(g) : -1;
+      }
     }
     if (piece >= 0) write_piece(piece & 1, piece >> 1);
   }
