@@ -38,9 +38,10 @@ template <int N>
 struct RingPos {
   int slot = 0;
   uint32_t phase = 0;
-  __device__ __forceinline__ void step() {
-    if (++slot == N) {
-      slot = 0;
+  __device__ __forceinline__ void step(int by = 1) {  // by < N
+    slot += by;
+    if (slot >= N) {
+      slot -= N;
       phase ^= 1u;
     }
   }

@@ -71,6 +71,15 @@ struct TrCfg {
   static_assert((kThreads / 32 + 4) * 8 <= 2 * 8 * NT * 4, "scratch fits in the sums");
   static constexpr int SMEM_BYTES = RED_OFF + 2 * 8 * NT * 4 + 1024;
   static_assert(Q_BYTES % 1024 == 0 && SMEM_BYTES <= 227 * 1024, "shared memory per CTA");
+  // The ring holds tiles in the order the tensor core uses them: K0 K1 V0 K2 V1
+  // K3 V2 ...: tile t's K is at position 2 t - 1 (0 for t = 0), its V at 2 t + 2.
+  struct KPos : RingPos<NSLOT> {
+    __device__ __forceinline__ void next(int t) { this->step(t == 0 ? 1 : 2); }  // from tile t to t + 1
+  };
+  struct VPos : RingPos<NSLOT> {
+    __device__ __forceinline__ VPos() { this->slot = 2; }
+    __device__ __forceinline__ void next() { this->step(2); }
+  };
   static constexpr uint32_t TMEM_COLS = NT == 64 ? 512 : 256;
   __device__ static constexpr uint32_t o_col(int parity) { return 128u + static_cast<uint32_t>(parity) * 2 * NT; }
 };
@@ -117,6 +126,7 @@ __device__ __forceinline__ float reduce8(const float* v, int lane) {
 // the negative tail; above it octic_fast2 is within 2.5e-6 s^2 <= 4e-5 of a
 // weight, and one special-function operation cheaper.
 constexpr float kTrTail = -4.0f;
+constexpr uint64_t kDrainNs = 1000000;  // 1 ms
 
 // Weights of 8 rows for one key, as bf16 pairs hi and lo with p = hi + lo, and
 // their sums. Bit e of `seen`: row e sees the key.
@@ -214,53 +224,55 @@ __global__ void __launch_bounds__(608, 1)
     // ------------------------------------------------------------------ TMA
     const bool is_v = warp == C::kTmaVWarp;
     KvPages pages(a);
-    int u = 0, qn = 0;
+    RingPos<C::NSLOT> pos;  // as KPos and VPos
+    if (is_v) pos.slot = 2;
+    int tile = 0, qn = 0;  // tile counts through all pieces of the CTA
     bool ok = true;
     while (ok && walk.next(a, p)) {
       if (!is_v && lane == 0) paged_meta_piece(a.meta, p);
       const int n = p.tiles > 0 ? p.t1 - p.t0 : 0;
       if (n == 0) continue;
-      const int qb = qn % C::QBUF;
-      if (!is_v && !(ok = __all_sync(0xffffffffu, mbar_wait(q_empty + qb, ((qn / C::QBUF) & 1) ^ 1, a.status,
-                                                            kDevTimeoutProducer))))
-        break;
-      if (!is_v && lane == 0) {
-        mbar_arrive_expect_tx(q_full + qb, C::KSUB * a.unit_rows * 128);
-        for (int h = 0; h < C::KSUB; ++h)
-          tma_load_4d(smem + C::Q_OFF + qb * C::Q_BYTES + h * C::QSUB_BYTES, &tm_q, q_full + qb, 64 * h, 0, p.h,
-                      p.r.tok0 + p.u * (a.unit_rows / a.G));
-      }
-      ++qn;
-      auto load = [&](int i, bool v, int page) {
-        const int slot = u++ % C::NSLOT;
-        if (v != is_v) return;  // the other warp's
-        if (!(ok = ok && __all_sync(0xffffffffu, mbar_wait(kv_empty + slot, (((u - 1) / C::NSLOT) & 1) ^ 1, a.status,
-                                                           kDevTimeoutProducer))))
-          return;
-        if (lane == 0) mbar_arrive_expect_tx(kv_full + slot, C::TILE_BYTES);
-        __syncwarp();
-        pages.template load<C::KSUB>(smem + C::KV_OFF + slot * C::TILE_BYTES, v ? &tm_v : &tm_k, kv_full + slot,
-                                     p, i, page);
-      };
-      int page[4];
+      int page[4];  // table entries are read ahead of their use
 #pragma unroll
       for (int i = 0; i < 4; ++i) page[i] = pages.page(a, p, i);
-      load(0, false, page[0]);
-      if (n > 1) load(1, false, page[1]);
-      for (int i = 0; ok && i < n; ++i) {
-        load(i, true, page[0]);
-        if (ok && i + 2 < n) load(i + 2, false, page[2]);
+      if (!is_v) {
+        const int qb = qn % C::QBUF;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(q_empty + qb, ((qn / C::QBUF) & 1) ^ 1, a.status,
+                                                     kDevTimeoutProducer))))
+          break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(q_full + qb, C::KSUB * a.unit_rows * 128);
+          for (int h = 0; h < C::KSUB; ++h)
+            tma_load_4d(smem + C::Q_OFF + qb * C::Q_BYTES + h * C::QSUB_BYTES, &tm_q, q_full + qb, 64 * h, 0, p.h,
+                        p.r.tok0 + p.u * (a.unit_rows / a.G));
+        }
+        ++qn;
+      }
+      for (int i = 0; i < n; ++i, ++tile) {
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(kv_empty + pos.slot, pos.phase ^ 1, a.status,
+                                                     kDevTimeoutProducer))))
+          break;
+        if (lane == 0) mbar_arrive_expect_tx(kv_full + pos.slot, C::TILE_BYTES);
+        __syncwarp();
+        pages.template load<C::KSUB>(smem + C::KV_OFF + pos.slot * C::TILE_BYTES, is_v ? &tm_v : &tm_k,
+                                     kv_full + pos.slot, p, i, page[0]);
+        pos.step(!is_v && tile == 0 ? 1 : 2);
         page[0] = page[1];
         page[1] = page[2];
         page[2] = page[3];
         page[3] = pages.page(a, p, i + 4);
       }
     }
-    // Do not leave the CTA while loads into its shared memory are in flight.
+    // Do not leave the CTA while loads into its shared memory are in flight:
+    // those of the ring's last round, whose slots nothing took after them. (The
+    // short budget is for a launch that failed, where that may not hold.)
     for (int x = qn - C::QBUF < 0 ? 0 : qn - C::QBUF; x < qn; ++x)
-      (void)mbar_wait(q_full + x % C::QBUF, (x / C::QBUF) & 1, nullptr, 0);
-    for (int x = u - C::NSLOT < 0 ? 0 : u - C::NSLOT; x < u; ++x)
-      (void)mbar_wait(kv_full + (x % C::NSLOT), (x / C::NSLOT) & 1, nullptr, 0);
+      (void)mbar_wait(q_full + x % C::QBUF, (x / C::QBUF) & 1, nullptr, 0, kDrainNs);
+    for (int x = tile - 1; x >= 0; --x) {
+      const int at = is_v ? 2 * x + 2 : x > 0 ? 2 * x - 1 : 0;
+      if (at <= 2 * tile - C::NSLOT) break;
+      (void)mbar_wait(kv_full + at % C::NSLOT, (at / C::NSLOT) & 1, nullptr, 0, kDrainNs);
+    }
   } else if (warp == C::kMmaWarp) {
     // ------------------------------------------------------------------ MMA
     constexpr uint32_t idesc_s = idesc_bf16_f32(128, NT, false);
@@ -283,55 +295,67 @@ __global__ void __launch_bounds__(608, 1)
         umma_ss(tmem + C::o_col(par), desc_add(vb, kk * 2048), desc_add(pd, kk * 2048), idesc_o,
                 (acc || kk > 0) ? 1u : 0u);
     };
-    int qn = 0, pc0 = 0, pc1 = 0, piece = -1;
-    RingPos<C::NSLOT> kv;
-    bool ok = true;
-    auto wait_kv = [&](const RingPos<C::NSLOT>& x) {
-      return __all_sync(0xffffffffu, mbar_wait(kv_full + x.slot, x.phase, a.status, kDevTimeoutMma));
+    // The tiles of all pieces are one stream: the scores run two tiles ahead of
+    // the outputs, also from one piece into the next, with a walk of their own.
+    PagedWalk swalk = walk;
+    typename C::KPos kpos;
+    typename C::VPos vpos;
+    bool ok = true, s_more = true;
+    int s_tile = 0, s_left = 0, s_qn = -1;
+    // Waits for the next tile's K (and its piece's Q): false when there is none.
+    auto wait_scores = [&]() {
+      while (s_left == 0) {
+        PagedPiece sp;
+        if (!s_more || !(s_more = swalk.next(a, sp))) return false;
+        s_left = uniform(sp.tiles > 0 ? sp.t1 - sp.t0 : 0);
+        if (s_left == 0) continue;
+        ++s_qn;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(q_full + s_qn % C::QBUF, (s_qn / C::QBUF) & 1, a.status,
+                                                     kDevTimeoutMma))))
+          return false;
+      }
+      return ok = __all_sync(0xffffffffu, mbar_wait(kv_full + kpos.slot, kpos.phase, a.status, kDevTimeoutMma));
     };
+    auto issue_scores = [&]() {  // one lane
+      issue_s(s_tile & 1, s_qn % C::QBUF, kpos.slot);
+      umma_commit(s_full + (s_tile & 1));
+      umma_commit(kv_empty + kpos.slot);
+      if (s_left == 1) umma_commit(q_empty + s_qn % C::QBUF);
+    };
+    auto scores_issued = [&]() {
+      kpos.next(s_tile);
+      ++s_tile;
+      --s_left;
+    };
+    int piece = -1, tile = 0;
+    for (int i = 0; i < 2 && wait_scores(); ++i) {
+      tc_fence_after();
+      if (elect_one()) issue_scores();
+      scores_issued();
+    }
     while (ok && walk.next(a, p)) {
       const int t0 = uniform(p.t0), n = uniform(p.tiles > 0 ? p.t1 : p.t0) - t0, len = uniform(p.r.len);
       ++piece;
-      if (n == 0) continue;
-      const int par = piece & 1, qb = qn % C::QBUF;
-      if (!(ok = __all_sync(0xffffffffu, mbar_wait(q_full + qb, (qn / C::QBUF) & 1, a.status, kDevTimeoutMma)))) break;
-      ++qn;
-      for (int i = 0; ok && i < min(2, n); ++i) {
-        if (!(ok = wait_kv(kv))) break;
-        tc_fence_after();
-        if (elect_one()) {
-          issue_s(i, qb, kv.slot);
-          umma_commit(s_full + i);
-          umma_commit(kv_empty + kv.slot);
-          if (i + 1 == n) umma_commit(q_empty + qb);
-        }
-        kv.step();
-      }
-      for (int i = 0; ok && i < n; ++i) {
-        const int g = i & 1, sv = kv.slot;
-        const bool more = i + 2 < n;
-        if (!(ok = wait_kv(kv))) break;
-        clear_v_tail<C::KSUB>(smem + C::KV_OFF + sv * C::TILE_BYTES, len - (t0 + i) * kPagedTile, a.page_shift, lane);
-        kv.step();
-        if (more && !(ok = wait_kv(kv))) break;
-        const int phase = g ? pc1++ : pc0++;
-        if (!(ok = __all_sync(0xffffffffu, mbar_wait(p_full + g, phase & 1, a.status, kDevTimeoutMma)))) break;
+      const int par = piece & 1;
+      for (int i = 0; ok && i < n; ++i, ++tile) {
+        const int g = tile & 1, slot = vpos.slot;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(kv_full + slot, vpos.phase, a.status, kDevTimeoutMma)))) break;
+        clear_v_tail<C::KSUB>(smem + C::KV_OFF + slot * C::TILE_BYTES, len - (t0 + i) * kPagedTile, a.page_shift, lane);
+        const bool scores = wait_scores();
+        if (!ok) break;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(p_full + g, (tile >> 1) & 1, a.status, kDevTimeoutMma)))) break;
         if (i == 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(o_empty + par, ((piece >> 1) & 1) ^ 1, a.status,
                                                                 kDevTimeoutMma))))
           break;
         tc_fence_after();
         if (elect_one()) {
-          issue_o(g, par, sv, i > 0);
-          umma_commit(kv_empty + sv);
+          issue_o(g, par, slot, i > 0);
+          umma_commit(kv_empty + slot);
           if (i + 1 == n) umma_commit(o_full + par);
-          if (more) {
-            issue_s(g, qb, kv.slot);
-            umma_commit(s_full + g);
-            umma_commit(kv_empty + kv.slot);
-            if (i + 3 == n) umma_commit(q_empty + qb);
-          }
+          if (scores) issue_scores();
         }
-        if (more) kv.step();
+        if (scores) scores_issued();
+        vpos.next();
       }
     }
     // Every MMA issued must finish before TMEM is released.
@@ -340,7 +364,7 @@ __global__ void __launch_bounds__(608, 1)
     __syncwarp();
   } else {
     // --------------------------------------------------- octic map + epilogue
-    const int g = warp >> 3;           // group: tiles g, g + 2, ... of a piece
+    const int g = warp >> 3;           // group: every other tile of the CTA
     const int half = (warp >> 2) & 1;  // its half of the rows
     const int sub = warp & 3;          // TMEM lane quarter
     constexpr int NH = C::NH;
@@ -353,7 +377,7 @@ __global__ void __launch_bounds__(608, 1)
       const int j = (r >> 3) & 7;
       st_shared_v4(p_row + (r >> 6) * C::SUB_BYTES + ((j ^ (krow & 7)) << 4), make_uint4(v[0], v[1], v[2], v[3]));
     };
-    int scnt = 0, piece = -1;
+    int scnt = 0, piece = -1, tiles = 0;  // tiles: of the pieces before
     int oc[2] = {0, 0};  // pieces with an O^T, by parity
     bool ok = true;
     // Outputs of a piece: O / (sum + sink), or the fragment.
@@ -428,7 +452,7 @@ __global__ void __launch_bounds__(608, 1)
       return p.t0 + i < p.t1 && key < p.r.len ? a.table[p.b * a.table_ld + (key >> a.page_shift)] : -1;
     };
     bool have = walk.next(a, p);
-    int next_entry = have ? entry(g) : -1;
+    int next_entry = have ? entry(g) : -1;  // of this group's first tile of the piece
     while (have) {
       ++piece;
       const int n = p.tiles > 0 ? p.t1 - p.t0 : 0;
@@ -439,7 +463,7 @@ __global__ void __launch_bounds__(608, 1)
       float sum[NH];
 #pragma unroll
       for (int i = 0; i < NH; ++i) sum[i] = 0.f;
-      for (int i = g; i < n && ok; i += 2) {
+      for (int i = (g ^ tiles) & 1; i < n && ok; i += 2) {
         const int key = (p.t0 + i) * kPagedTile + krow;
         const bool in = next_entry >= 0 && next_entry < a.num_pages;
         next_entry = entry(i + 2);
@@ -509,9 +533,10 @@ __global__ void __launch_bounds__(608, 1)
       // The next piece's first table entry is under way while the outputs are
       // written (with 64 rows there are no registers to hold it).
       constexpr bool kAhead = NT < 64;
+      tiles += n;
       if (kAhead) {
         have = walk.next(a, p);
-        next_entry = have ? entry(g) : -1;
+        next_entry = have ? entry((g ^ tiles) & 1) : -1;
       }
       if (piece > 0) write_piece(par ^ 1, (piece - 1) >> 1);
       d_rows = rows;
@@ -520,7 +545,7 @@ __global__ void __launch_bounds__(608, 1)
       d_kind = kind;
       if (!kAhead) {
         have = walk.next(a, p);
-        next_entry = have ? entry(g) : -1;
+        next_entry = have ? entry((g ^ tiles) & 1) : -1;
       }
     }
     if (piece >= 0) write_piece(piece & 1, piece >> 1);
