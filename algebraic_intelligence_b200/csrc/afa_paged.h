@@ -37,7 +37,7 @@ struct PagedArgs {
 bool paged_tc_supported(const PagedArgs& a, int dtype);
 // The tensor-core kernel's launch shape: query rows per work unit, CTAs.
 int paged_tc_unit_rows(int G);
-// Query rows per unit of the transposed kernel for this batch (16, 32 or 64; a
+// Query rows per unit of the transposed kernel for this batch (16 or 32; a
 // unit has the largest multiple of G up to it), or 0 when the rows a request
 // has on average are too many for it.
 int paged_tr_rows(int B, int T, int G);

@@ -6,7 +6,7 @@
 //   O^T += V^T P^T  M = head_dim,  N = NT, over the tile's 128 keys
 //
 // The query rows are the narrow side of both products, so the tensor core and
-// the octic map work on NT (16, 32 or 64) rows and not on the 128 that a row
+// the octic map work on NT (16 or 32) rows and not on the 128 that a row
 // tile of the other kernel has: a thread owns one key and maps NT scores, and
 // every warp has the same share whatever the number of rows. What is left is
 // the cache's bytes. That leaves room for exactness: a weight enters the second
@@ -57,12 +57,11 @@ struct TrCfg {
   static constexpr int TILE_BYTES = KSUB * SUB_BYTES;
   static constexpr int QSUB_BYTES = NT * 128;
   static constexpr int Q_BYTES = KSUB * QSUB_BYTES;
-  static constexpr int P_BYTES = (2 * NT + 63) / 64 * SUB_BYTES;  // 128 keys x 64-row blocks
+  static constexpr int P_BYTES = SUB_BYTES;  // 128 keys x 64 columns: hi and lo of up to 32 rows
   static constexpr int Q_OFF = 0;
-  static constexpr int QBUF = NT == 64 && HD == 128 ? 1 : 2;  // query buffers: what shared memory leaves
-  static constexpr int P_OFF = QBUF * Q_BYTES;
+  static constexpr int P_OFF = 2 * Q_BYTES;
   static constexpr int KV_OFF = P_OFF + 2 * P_BYTES;
-  static constexpr int NSLOT = HD == 128 ? (NT == 64 ? 4 : 5) : (NT == 64 ? 7 : 8);
+  static constexpr int NSLOT = HD == 128 ? 5 : 8;
   static constexpr int BAR_OFF = KV_OFF + NSLOT * TILE_BYTES;
   static constexpr int NBAR = 4 + 2 * NSLOT + 2 + 2 + 2 + 2 + 2 + 1;
   static constexpr int TMEM_OFF = BAR_OFF + NBAR * 8;
@@ -80,7 +79,7 @@ struct TrCfg {
     __device__ __forceinline__ VPos() { this->slot = 2; }
     __device__ __forceinline__ void next() { this->step(2); }
   };
-  static constexpr uint32_t TMEM_COLS = NT == 64 ? 512 : 256;
+  static constexpr uint32_t TMEM_COLS = 256;
   __device__ static constexpr uint32_t o_col(int parity) { return 128u + static_cast<uint32_t>(parity) * 2 * NT; }
 };
 
@@ -90,17 +89,13 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
                : "r"(taddr));
 }
 
-// N columns (1, 2 or 4) of this thread's lane.
+// N columns (1 or 2) of this thread's lane.
 template <int N>
 __device__ __forceinline__ void tmem_ld_few(uint32_t taddr, uint32_t (&r)[N]) {
   if constexpr (N == 1)
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r[0]) : "r"(taddr));
-  else if constexpr (N == 2)
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(taddr));
   else
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(taddr));
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(taddr));
 }
 
 // Sums of 8 values over the warp's lanes: lane l returns value l / 4's.
@@ -236,8 +231,8 @@ __global__ void __launch_bounds__(608, 1)
 #pragma unroll
       for (int i = 0; i < 4; ++i) page[i] = pages.page(a, p, i);
       if (!is_v) {
-        const int qb = qn % C::QBUF;
-        if (!(ok = __all_sync(0xffffffffu, mbar_wait(q_empty + qb, ((qn / C::QBUF) & 1) ^ 1, a.status,
+        const int qb = qn & 1;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(q_empty + qb, ((qn >> 1) & 1) ^ 1, a.status,
                                                      kDevTimeoutProducer))))
           break;
         if (lane == 0) {
@@ -266,8 +261,8 @@ __global__ void __launch_bounds__(608, 1)
     // Do not leave the CTA while loads into its shared memory are in flight:
     // those of the ring's last round, whose slots nothing took after them. (The
     // short budget is for a launch that failed, where that may not hold.)
-    for (int x = qn - C::QBUF < 0 ? 0 : qn - C::QBUF; x < qn; ++x)
-      (void)mbar_wait(q_full + x % C::QBUF, (x / C::QBUF) & 1, nullptr, 0, kDrainNs);
+    for (int x = qn - 2 < 0 ? 0 : qn - 2; x < qn; ++x)
+      (void)mbar_wait(q_full + (x & 1), (x >> 1) & 1, nullptr, 0, kDrainNs);
     for (int x = tile - 1; x >= 0; --x) {
       const int at = is_v ? 2 * x + 2 : x > 0 ? 2 * x - 1 : 0;
       if (at <= 2 * tile - C::NSLOT) break;
@@ -310,17 +305,17 @@ __global__ void __launch_bounds__(608, 1)
         s_left = uniform(sp.tiles > 0 ? sp.t1 - sp.t0 : 0);
         if (s_left == 0) continue;
         ++s_qn;
-        if (!(ok = __all_sync(0xffffffffu, mbar_wait(q_full + s_qn % C::QBUF, (s_qn / C::QBUF) & 1, a.status,
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(q_full + (s_qn & 1), (s_qn >> 1) & 1, a.status,
                                                      kDevTimeoutMma))))
           return false;
       }
       return ok = __all_sync(0xffffffffu, mbar_wait(kv_full + kpos.slot, kpos.phase, a.status, kDevTimeoutMma));
     };
     auto issue_scores = [&]() {  // one lane
-      issue_s(s_tile & 1, s_qn % C::QBUF, kpos.slot);
+      issue_s(s_tile & 1, s_qn & 1, kpos.slot);
       umma_commit(s_full + (s_tile & 1));
       umma_commit(kv_empty + kpos.slot);
-      if (s_left == 1) umma_commit(q_empty + s_qn % C::QBUF);
+      if (s_left == 1) umma_commit(q_empty + (s_qn & 1));
     };
     auto scores_issued = [&]() {
       kpos.next(s_tile);
@@ -371,11 +366,10 @@ __global__ void __launch_bounds__(608, 1)
     const uint32_t lane_off = static_cast<uint32_t>(sub * 32) << 16;
     const int krow = sub * 32 + lane;  // this thread's key of a tile
     const uint32_t p_row = smem_u32(smem + C::P_OFF + g * C::P_BYTES + krow * 128);
-    // Rows [r, r + 8) of this thread's key: 16-byte chunk j of key row k lies at
-    // (j ^ (k % 8)) * 16 of the row's 128 bytes in its 64-row block.
+    // Columns [r, r + 8) of this thread's key: 16-byte chunk j of key row k lies
+    // at (j ^ (k % 8)) * 16 of the row's 128 bytes.
     auto put = [&](int r, const uint32_t (&v)[4]) {
-      const int j = (r >> 3) & 7;
-      st_shared_v4(p_row + (r >> 6) * C::SUB_BYTES + ((j ^ (krow & 7)) << 4), make_uint4(v[0], v[1], v[2], v[3]));
+      st_shared_v4(p_row + (((r >> 3) ^ (krow & 7)) << 4), make_uint4(v[0], v[1], v[2], v[3]));
     };
     int scnt = 0, piece = -1, tiles = 0;  // tiles: of the pieces before
     int oc[2] = {0, 0};  // pieces with an O^T, by parity
@@ -468,7 +462,7 @@ __global__ void __launch_bounds__(608, 1)
         const bool in = next_entry >= 0 && next_entry < a.num_pages;
         next_entry = entry(i + 2);
         // Rows that see this thread's key.
-        unsigned long long seen = in ? ~0ull : 0ull;
+        unsigned seen = in ? ~0u : 0u;
         const int at = key - prefix;
         if (in && at >= 0) {
           if (a.anc) {
@@ -477,11 +471,11 @@ __global__ void __launch_bounds__(608, 1)
             if (w < a.words)
               for (int j = 0; j * a.G < rows; ++j) {
                 const unsigned word = a.anc[static_cast<long long>(p.r.tok0 + tok_u + j) * a.anc_ld + w];
-                if ((word >> (at & 31)) & 1u) seen |= ((1ull << (a.G - 1)) * 2 - 1) << (j * a.G);
+                if ((word >> (at & 31)) & 1u) seen |= ((1u << (a.G - 1)) * 2u - 1u) << (j * a.G);
               }
           } else {
             const long long first = static_cast<long long>(at) * a.G - row0;  // first row of token `at`
-            seen = first <= 0 ? ~0ull : first >= 64 ? 0ull : ~0ull << first;
+            seen = first <= 0 ? ~0u : first >= 32 ? 0u : ~0u << first;
           }
         }
         ok = __all_sync(0xffffffffu, mbar_wait(s_full + g, scnt & 1, a.status, kDevTimeoutSoftmax));
@@ -492,15 +486,13 @@ __global__ void __launch_bounds__(608, 1)
         if (mine) {
           const uint32_t s_tm = tmem + g * NT + lane_off + half * NH;
           uint32_t sv[NH];
-          if constexpr (NH == 32)
-            tmem_ld32(s_tm, sv);
-          else if constexpr (NH == 16)
+          if constexpr (NH == 16)
             tmem_ld16(s_tm, sv);
           else
             tmem_ld8(s_tm, sv);
           tmem_ld_wait();
-          const unsigned word = static_cast<unsigned>(seen >> (half * NH));
-          const bool all_seen = __all_sync(0xffffffffu, seen == ~0ull);
+          const unsigned word = seen >> (half * NH);
+          const bool all_seen = __all_sync(0xffffffffu, seen == ~0u);
 #pragma unroll
           for (int c = 0; c < NH; c += 8) {
             uint32_t hi[4], lo[4];
@@ -531,22 +523,15 @@ __global__ void __launch_bounds__(608, 1)
       const int tok = p.r.tok0 + tok_u, head = p.h;
       const int kind = (p.whole() ? 1 : 0) | paged_frag_slot(p) << 1 | (n > 0 ? 4 : 0);
       // The next piece's first table entry is under way while the outputs are
-      // written (with 64 rows there are no registers to hold it).
-      constexpr bool kAhead = NT < 64;
+      // written.
       tiles += n;
-      if (kAhead) {
-        have = walk.next(a, p);
-        next_entry = have ? entry((g ^ tiles) & 1) : -1;
-      }
+      have = walk.next(a, p);
+      next_entry = have ? entry((g ^ tiles) & 1) : -1;
       if (piece > 0) write_piece(par ^ 1, (piece - 1) >> 1);
       d_rows = rows;
       d_tok = tok;
       d_h = head;
       d_kind = kind;
-      if (!kAhead) {
-        have = walk.next(a, p);
-        next_entry = have ? entry((g ^ tiles) & 1) : -1;
-      }
     }
     if (piece >= 0) write_piece(piece & 1, piece >> 1);
   }
@@ -586,20 +571,17 @@ cudaError_t launch_nt(const PagedArgs& a, int ctas, cudaStream_t stream, const c
 
 template <int HD>
 cudaError_t launch_hd(const PagedArgs& a, int nt, int ctas, cudaStream_t stream, const char** detail) {
-  switch (nt) {
-    case 16: return launch_nt<HD, 16>(a, ctas, stream, detail);
-    case 32: return launch_nt<HD, 32>(a, ctas, stream, detail);
-    default: return launch_nt<HD, 64>(a, ctas, stream, detail);
-  }
+  return nt == 16 ? launch_nt<HD, 16>(a, ctas, stream, detail) : launch_nt<HD, 32>(a, ctas, stream, detail);
 }
 
 }  // namespace
 
+// Measured against the row-tile kernel over 64 x 8192 keys of 8 heads: 32 rows
+// 264 us (row tiles 320), 64 rows, with a variant that had twice the columns,
+// 348 (322); over 256 x 200 keys 64 rows 203 (117).
 int paged_tr_rows(int B, int T, int G) {
   const long long rows = (static_cast<long long>(T) + B - 1) / B * G;
-  for (int nt : {16, 32, 64})
-    if (rows <= nt) return nt;
-  return 0;
+  return rows <= 16 ? 16 : rows <= 32 ? 32 : 0;
 }
 
 cudaError_t launch_paged_tr(const PagedArgs& a, int nt, int ctas, cudaStream_t stream, const char** detail) {
