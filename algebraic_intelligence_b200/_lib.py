@@ -124,7 +124,8 @@ def accum_dtype(dt: torch.dtype) -> torch.dtype:
 def stream_ptr(device: torch.device) -> int:
     # The raw handle of torch.cuda.current_stream(device), without the Stream
     # object around it (4 us of host time per call).
-    return torch._C._cuda_getCurrentRawStream(device.index)
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 @functools.lru_cache(maxsize=4096)
