@@ -36,11 +36,13 @@ constexpr int kSimtThreads = 256;
 // like signs only, correctly rounded root and quotient, so rho is within 1.5
 // half steps for every s and float32 weights within 16 (octic_ref's reciprocal
 // root alone is off by up to 2 steps).
+__device__ __forceinline__ float recip(float x) { return __frcp_rn(x); }
+__device__ __forceinline__ double recip(double x) { return __drcp_rn(x); }
 template <typename A>
 __device__ __forceinline__ A octic_even(A s) {
   const A t = s < A(0) ? -s : s;
   A rho = t + sqrt(fma(s, s, A(1)));
-  if (s < A(0)) rho = A(1) / rho;
+  if (s < A(0)) rho = recip(rho);
   const A k2 = rho * rho, k4 = k2 * k2;
   return k4 * k4;
 }
@@ -52,37 +54,49 @@ struct alignas(16) Quad {
   A x[N];
 };
 
-// ROWS query rows x BN keys per step. 256 threads as RY x CX: thread (ty, tx)
-// owns scores (ty + RY i, tx + CX j) and, of outputs, the channels of 16 bytes
-// number tx + CX j of the same rows. Shared memory holds rows of DMAX padded by
-// 16 bytes, read 16 bytes at a time: a quarter warp's reads fall on different
-// banks or are one broadcast. Bound by those reads and the FMAs (8 or 32 rows
-// share every key); several CTAs per SM cover the loads' latency. Sums run over
-// BN keys in registers of their own before they join the row's, which keeps
-// float32 results near 1e-7 at any length.
-template <typename T, typename A, int ROWS, int BN, int DMAX>
+// ROWS query rows x BN keys per step, 256 threads. Scores: a warp is LY rows x
+// LX keys, a thread owns TR x TC of them; outputs: a thread owns RP rows of OC
+// groups of 16 bytes of channels (with KS = 2 one of two halves of the keys as
+// well), a warp 4 rows x 8 groups. Both ways a quarter warp's 16-byte reads of
+// shared memory fall on different banks or are one broadcast, and there are few
+// of them for each FMA (6 to 32, 8 to 64 with 32 rows): the FMAs bound 32 rows,
+// the cache's bytes 8. Shared rows are DMAX channels padded by 16 bytes; several
+// CTAs per SM cover the loads' latency. Sums run over BN keys in registers of
+// their own before they join the row's, which keeps float32 results near 1e-7 at
+// any length.
+template <typename A, int ROWS, int BN, int DMAX>
 struct SimtCfg {
-  static constexpr int RY = ROWS < 16 ? ROWS : 16, CX = kSimtThreads / RY;
-  static constexpr int TR = ROWS / RY, TC = BN / CX;
   static constexpr int V = Quad<A>::N;
+  static constexpr int LX = ROWS == 8 && BN == 64 ? 8 : 4, LY = 32 / LX;
+  static constexpr int TR = ROWS / LY, TC = BN / (8 * LX);
+  static constexpr int CG = DMAX / V < 64 ? DMAX / V : 64, OC = DMAX / V / CG;  // channel groups across threads
+  static constexpr int RG = kSimtThreads / CG;
+  static constexpr int KS = RG > ROWS ? RG / ROWS : 1, RP = RG > ROWS ? 1 : ROWS / RG;
   static constexpr int LD = DMAX + V, PLD = BN + V;
-  static constexpr int OC = (DMAX / V + CX - 1) / CX;
   static constexpr size_t kSmem = sizeof(A) * (static_cast<size_t>(ROWS + 2 * BN) * LD + static_cast<size_t>(ROWS) * PLD);
+  static_assert(TC >= 1 && TR >= 1 && KS <= 2 && CG % 8 == 0, "thread mapping");
+  static_assert(KS == 1 || static_cast<size_t>(ROWS) * DMAX <= static_cast<size_t>(BN) * LD, "halves meet in the K tile");
 };
 
 template <typename T, typename A, int ROWS, int BN, int DMAX>
 __global__ void __launch_bounds__(kSimtThreads) afa_paged_simt_kernel(const __grid_constant__ PagedArgs a) {
-  using C = SimtCfg<T, A, ROWS, BN, DMAX>;
-  constexpr int RY = C::RY, CX = C::CX, TR = C::TR, TC = C::TC, V = C::V, LD = C::LD, PLD = C::PLD, OC = C::OC;
+  using C = SimtCfg<A, ROWS, BN, DMAX>;
+  constexpr int V = C::V, LX = C::LX, LY = C::LY, TR = C::TR, TC = C::TC, OC = C::OC, RP = C::RP, LD = C::LD,
+                PLD = C::PLD;
   using Q4 = Quad<A>;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   __shared__ long long share_sm[kSimtThreads / 32 + 4];
   __shared__ long long k_row[BN], v_row[BN];  // offsets of the step's cache rows; below 0: none
+  __shared__ A sums[8][ROWS];                 // row sums, by warp
   A* Qs = reinterpret_cast<A*>(smem_raw);
   A* Ks = Qs + ROWS * LD;
   A* Vs = Ks + BN * LD;
   A* Ps = Vs + BN * LD;
-  const int tid = threadIdx.x, tx = tid % CX, ty = tid / CX, D = a.D;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, D = a.D;
+  const int kx = warp * LX + lane % LX, ry = lane / LX;  // scores: keys kx + 8 LX j, rows ry + LY i
+  constexpr int WC = C::CG / 8;                          // warps along the channels
+  const int cg = lane % 8 + 8 * (warp % WC), rg = lane / 8 + 4 * (warp / WC);
+  const int ks = C::KS == 2 ? rg / ROWS : 0, ro = C::KS == 2 ? rg % ROWS : rg;  // outputs: rows ro + RG i
   const int dv = (D + V - 1) / V;  // 16-byte channel groups; the last is padded with zeros
   const T* q = static_cast<const T*>(a.q);
   T* out = static_cast<T*>(a.out);
@@ -127,18 +141,16 @@ __global__ void __launch_bounds__(kSimtThreads) afa_paged_simt_kernel(const __gr
       }
       *reinterpret_cast<Q4*>(Qs + r * LD + c * V) = fetch(src, c);
     }
-    int node[TR];
-    A o[TR][OC][V], rs[TR];
+    A rs[TR];
+    A o[RP][OC][V];
 #pragma unroll
-    for (int i = 0; i < TR; ++i) {
-      const int r = ty + RY * i;
-      node[i] = r < rows ? (row0 + r) / a.G : -1;
-      rs[i] = A(0);
+    for (int i = 0; i < TR; ++i) rs[i] = A(0);
+#pragma unroll
+    for (int i = 0; i < RP; ++i)
 #pragma unroll
       for (int j = 0; j < OC; ++j)
 #pragma unroll
         for (int e = 0; e < V; ++e) o[i][j][e] = A(0);
-    }
     const int k_end = p.tiles == 0 ? 0 : min(p.t1 * kPagedTile, p.r.len);
     const int prefix = p.r.len - p.r.n;
     for (int k0 = p.t0 * kPagedTile; k0 < k_end; k0 += BN) {
@@ -164,10 +176,10 @@ __global__ void __launch_bounds__(kSimtThreads) afa_paged_simt_kernel(const __gr
       for (int i = tid; i < BN * dv; i += kSimtThreads) {
         const int r = i / dv, c = i - r * dv;
         const long long ko = k_row[r], vo = v_row[r];
-        const Q4 kx = fetch(ko < 0 ? nullptr : static_cast<const T*>(a.k) + ko, c);
-        const Q4 vx = fetch(ko < 0 ? nullptr : static_cast<const T*>(a.v) + vo, c);
-        *reinterpret_cast<Q4*>(Ks + r * LD + c * V) = kx;
-        *reinterpret_cast<Q4*>(Vs + r * LD + c * V) = vx;
+        const Q4 x = fetch(ko < 0 ? nullptr : static_cast<const T*>(a.k) + ko, c);
+        const Q4 y = fetch(ko < 0 ? nullptr : static_cast<const T*>(a.v) + vo, c);
+        *reinterpret_cast<Q4*>(Ks + r * LD + c * V) = x;
+        *reinterpret_cast<Q4*>(Vs + r * LD + c * V) = y;
       }
       __syncthreads();
       A s[TR][TC];
@@ -179,9 +191,9 @@ __global__ void __launch_bounds__(kSimtThreads) afa_paged_simt_kernel(const __gr
       for (int c = 0; c < dv; ++c) {
         Q4 x[TR], y[TC];
 #pragma unroll
-        for (int i = 0; i < TR; ++i) x[i] = *reinterpret_cast<const Q4*>(Qs + (ty + RY * i) * LD + c * V);
+        for (int i = 0; i < TR; ++i) x[i] = *reinterpret_cast<const Q4*>(Qs + (ry + LY * i) * LD + c * V);
 #pragma unroll
-        for (int j = 0; j < TC; ++j) y[j] = *reinterpret_cast<const Q4*>(Ks + (tx + CX * j) * LD + c * V);
+        for (int j = 0; j < TC; ++j) y[j] = *reinterpret_cast<const Q4*>(Ks + (kx + 8 * LX * j) * LD + c * V);
 #pragma unroll
         for (int e = 0; e < V; ++e)
 #pragma unroll
@@ -191,44 +203,40 @@ __global__ void __launch_bounds__(kSimtThreads) afa_paged_simt_kernel(const __gr
       }
 #pragma unroll
       for (int i = 0; i < TR; ++i) {
-        A part = A(0);
+        const int r = ry + LY * i;
 #pragma unroll
-        for (int w = 0; w < (BN + 31) / 32; ++w) {
-          const unsigned seen = all_seen ? 0xffffffffu : node[i] < 0 ? 0u : paged_seen(a, p.r, node[i], k0 + 32 * w);
-#pragma unroll
-          for (int j = 0; j < TC; ++j) {
-            const int c = tx + CX * j;
-            if ((CX * j) / 32 != w) continue;
-            const bool in = ((seen >> (c & 31)) & 1u) && (all_seen || k_row[c] >= 0);
-            const A pr = in ? octic_even(s[i][j] * scale) : A(0);
-            part += pr;
-            Ps[(ty + RY * i) * PLD + c] = pr;
-          }
+        for (int j = 0; j < TC; ++j) {
+          const int c = kx + 8 * LX * j;
+          bool in = all_seen;
+          if (!all_seen && r < rows && k_row[c] >= 0)
+            in = (paged_seen(a, p.r, (row0 + r) / a.G, k0 + (c & ~31)) >> (c & 31)) & 1u;
+          const A pr = in ? octic_even(s[i][j] * scale) : A(0);
+          rs[i] += pr;
+          Ps[r * PLD + c] = pr;
         }
-        rs[i] += part;
       }
       __syncthreads();
-      A ot[TR][OC][V];
+      A ot[RP][OC][V];
 #pragma unroll
-      for (int i = 0; i < TR; ++i)
+      for (int i = 0; i < RP; ++i)
 #pragma unroll
         for (int j = 0; j < OC; ++j)
 #pragma unroll
           for (int e = 0; e < V; ++e) ot[i][j][e] = A(0);
 #pragma unroll 2
-      for (int kk = 0; kk < BN; kk += V) {
-        Q4 pv[TR];
+      for (int kk = ks * V; kk < BN; kk += C::KS * V) {
+        Q4 pv[RP];
 #pragma unroll
-        for (int i = 0; i < TR; ++i) pv[i] = *reinterpret_cast<const Q4*>(Ps + (ty + RY * i) * PLD + kk);
+        for (int i = 0; i < RP; ++i) pv[i] = *reinterpret_cast<const Q4*>(Ps + (ro + C::RG * i) * PLD + kk);
 #pragma unroll
         for (int j = 0; j < OC; ++j) {
-          const int c = tx + CX * j;
+          const int c = cg + C::CG * j;
           if (c < dv) {
 #pragma unroll
             for (int y = 0; y < V; ++y) {
               const Q4 vv = *reinterpret_cast<const Q4*>(Vs + (kk + y) * LD + c * V);
 #pragma unroll
-              for (int i = 0; i < TR; ++i)
+              for (int i = 0; i < RP; ++i)
 #pragma unroll
                 for (int e = 0; e < V; ++e) ot[i][j][e] = fma(pv[i].x[y], vv.x[e], ot[i][j][e]);
             }
@@ -236,39 +244,57 @@ __global__ void __launch_bounds__(kSimtThreads) afa_paged_simt_kernel(const __gr
         }
       }
 #pragma unroll
-      for (int i = 0; i < TR; ++i)
+      for (int i = 0; i < RP; ++i)
 #pragma unroll
         for (int j = 0; j < OC; ++j)
 #pragma unroll
           for (int e = 0; e < V; ++e) o[i][j][e] += ot[i][j][e];
     }
-    // The CX threads of a row are neighbours in a warp.
+    // Row sums: over the lanes of a row, then over the warps in order.
 #pragma unroll
     for (int i = 0; i < TR; ++i) {
 #pragma unroll
-      for (int off = CX / 2; off > 0; off >>= 1) rs[i] += __shfl_xor_sync(0xffffffffu, rs[i], off);
-      const int r = ty + RY * i;
-      if (r >= rows) continue;
+      for (int off = LX / 2; off > 0; off >>= 1) rs[i] += __shfl_xor_sync(0xffffffffu, rs[i], off);
+      if (lane % LX == 0) sums[warp][ry + LY * i] = rs[i];
+    }
+    if (C::KS == 2) {  // the second half of the keys, through the K tile
+      if (ks == 1)
+#pragma unroll
+        for (int e = 0; e < V; ++e) Ks[ro * DMAX + cg * V + e] = o[0][0][e];
+    }
+    __syncthreads();
+    if (C::KS == 2) {
+      if (ks == 0)
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[0][0][e] += Ks[ro * DMAX + cg * V + e];
+    }
+    const bool whole = p.whole();
+    A* f = frag + static_cast<long long>(paged_frag_slot(p)) * a.frag_rows * (D + 1);
+#pragma unroll
+    for (int i = 0; i < RP; ++i) {
+      const int r = ro + C::RG * i;
+      if (r >= rows || ks != 0) continue;
+      A total = A(0);
+#pragma unroll
+      for (int w = 0; w < 8; ++w) total += sums[w][r];
       const int tok = (row0 + r) / a.G;
       const long long orow = (static_cast<long long>(p.r.tok0) + tok) * a.Hkv * a.G +
                              static_cast<long long>(p.h) * a.G + (row0 + r - tok * a.G);
-      const bool whole = p.whole();
-      const A denom = rs[i] + sink;
-      A* f = frag + static_cast<long long>(paged_frag_slot(p)) * a.frag_rows * (D + 1);
+      const A denom = total + sink;
 #pragma unroll
       for (int j = 0; j < OC; ++j)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const int c = (tx + CX * j) * V + e;
+          const int c = (cg + C::CG * j) * V + e;
           if (c >= D) continue;
           if (whole)
             out[orow * D + c] = from_acc<T>(denom > A(0) ? o[i][j][e] / denom : A(0));
           else
             f[static_cast<long long>(r) * D + c] = o[i][j][e];
         }
-      if (tx == 0) {
+      if (cg == 0) {
         if (!whole)
-          f[static_cast<long long>(a.frag_rows) * D + r] = rs[i];
+          f[static_cast<long long>(a.frag_rows) * D + r] = total;
         else if (dtot)
           dtot[orow] = denom;
       }
@@ -340,25 +366,37 @@ __global__ void __launch_bounds__(kCombineWarps * 32) paged_combine_kernel(const
   }
 }
 
+// CTAs of a launch per SM: one of the tensor-core kernels fills an SM, of the
+// CUDA-core kernel up to four fit (float32, 64 channels).
+constexpr int kMaxSms = 148, kSimtPerSm = 4;
+
+// `ctas` comes as the number of SMs and leaves as the number of CTAs: all that
+// are resident at once, since equal shares in a second round would take as long
+// again.
 template <typename T, typename A, int ROWS, int BN, int DMAX>
-cudaError_t launch_simt(const PagedArgs& a, int ctas, cudaStream_t stream) {
-  constexpr size_t smem = SimtCfg<T, A, ROWS, BN, DMAX>::kSmem;
-  static_assert(smem <= 227 * 1024, "shared memory per CTA");
+cudaError_t launch_simt(const PagedArgs& a, int* ctas, cudaStream_t stream) {
+  constexpr size_t smem = SimtCfg<A, ROWS, BN, DMAX>::kSmem;
+  static_assert(smem <= 220 * 1024, "shared memory per CTA");
   static PerDeviceOnce setup;
+  static int per_sm[kMaxDevices] = {};
   auto kern = afa_paged_simt_kernel<T, A, ROWS, BN, DMAX>;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess)
     e = setup.run(dev, [&] {
-      return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+      const cudaError_t r =
+          cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+      return r != cudaSuccess ? r
+                              : cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm[dev], kern, kSimtThreads, smem);
     });
   if (e != cudaSuccess) return e;
-  kern<<<ctas, kSimtThreads, smem, stream>>>(a);
+  *ctas *= std::max(1, std::min(per_sm[dev], kSimtPerSm));
+  kern<<<*ctas, kSimtThreads, smem, stream>>>(a);
   return cudaGetLastError();
 }
 
 template <typename T, typename A, int ROWS>
-cudaError_t launch_simt_rows(const PagedArgs& a, int ctas, cudaStream_t stream) {
+cudaError_t launch_simt_rows(const PagedArgs& a, int* ctas, cudaStream_t stream) {
   if constexpr (sizeof(A) == 8) {
     if (a.D <= 128) return launch_simt<T, A, ROWS, 32, 128>(a, ctas, stream);
     return launch_simt<T, A, ROWS, 32, 256>(a, ctas, stream);
@@ -370,7 +408,7 @@ cudaError_t launch_simt_rows(const PagedArgs& a, int ctas, cudaStream_t stream) 
 }
 
 template <typename T, typename A>
-cudaError_t launch_simt_type(const PagedArgs& a, int ctas, cudaStream_t stream) {
+cudaError_t launch_simt_type(const PagedArgs& a, int* ctas, cudaStream_t stream) {
   return a.unit_rows == 8 ? launch_simt_rows<T, A, 8>(a, ctas, stream) : launch_simt_rows<T, A, 32>(a, ctas, stream);
 }
 
@@ -410,10 +448,6 @@ int sm_count() {
       setup.run(dev, [&] { return cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev); });
   return e == cudaSuccess ? count[dev] : 0;
 }
-
-// CTAs of a launch per SM: one of the tensor-core kernels fills an SM, of the
-// CUDA-core kernel up to four fit (float32, 64 channels).
-constexpr int kMaxSms = 148, kSimtPerSm = 4;
 
 // Rows of a CUDA-core unit: 8 where requests have no more on average (single
 // tokens), else 32.
@@ -538,7 +572,6 @@ extern "C" int afa_paged(const void* q, const long long* q_strides, const void* 
     for (const void* x : {a.q, a.k, a.v}) a.wide = a.wide && reinterpret_cast<uintptr_t>(x) % run == 0;
     for (long long s : {a.q_st, a.q_sh, a.k_sp, a.k_sh, a.k_sr, a.v_sp, a.v_sh, a.v_sr})
       a.wide = a.wide && s * static_cast<long long>(es) % static_cast<long long>(run) == 0;
-    ctas *= kSimtPerSm;
   }
   a.frag_rows = frag_rows_of(a.unit_rows, tokens, a.G);
   const char* detail = "";
@@ -546,9 +579,9 @@ extern "C" int afa_paged(const void* q, const long long* q_strides, const void* 
   if (tc) {
     e = nt ? launch_paged_tr(a, nt, ctas, st, &detail) : launch_paged_tc(a, ctas, st, &detail);
   } else switch (dtype) {
-    case kF64: e = launch_simt_type<double, double>(a, ctas, st); break;
-    case kF32: e = launch_simt_type<float, float>(a, ctas, st); break;
-    default: e = launch_simt_type<__nv_bfloat16, float>(a, ctas, st); break;
+    case kF64: e = launch_simt_type<double, double>(a, &ctas, st); break;
+    case kF32: e = launch_simt_type<float, float>(a, &ctas, st); break;
+    default: e = launch_simt_type<__nv_bfloat16, float>(a, &ctas, st); break;
   }
   if (e == cudaSuccess) {
     switch (dtype) {
