@@ -252,7 +252,8 @@ extern "C" int afa_paged_plan(int* block_table, const int* page_counts, const in
                               int page_size, int num_free, int max_tokens, int nodes, void* stream) {
   using namespace afa;
   if (batch <= 0 || batch > kPlanMaxBatch) return invalid("afa_paged_plan: batch must be in [1, 4096]");
-  if (table_cols <= 0 || num_free <= 0 || max_tokens < 0) return invalid("afa_paged_plan: invalid shape");
+  if (table_cols <= 0 || num_free <= 0 || max_tokens < 0 || max_tokens > (1 << 30))
+    return invalid("afa_paged_plan: invalid shape");
   if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)) != 0)
     return invalid("page_size must be a power of two from 16 to 256");
   if (static_cast<long long>(table_cols) * page_size > INT_MAX - 65536 ||

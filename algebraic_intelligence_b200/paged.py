@@ -18,7 +18,9 @@ its requests append a prompt, a token or a tree of drafted tokens:
                     the next ``paged_plan`` takes back the other nodes' pages
 
 The tensors are CUDA tensors on one device; calls run on its current stream.
-The caches, the block table and the free stack are updated in place.
+The caches, the block table and the free stack are updated in place. Make the
+first call of each on a device before any stream capture: it sets kernel
+attributes and resolves the device status word.
 """
 from __future__ import annotations
 
@@ -130,8 +132,8 @@ def paged_plan(block_table, page_counts, seq_lens, new_lens, free_pages, free_co
     if b > 4096:
         raise ValueError("paged_plan: batch must be in [1, 4096]")
     _check_page_size(page_size)
-    if not isinstance(max_tokens, int) or max_tokens < 0:
-        raise ValueError("max_tokens must be a nonnegative integer")
+    if not isinstance(max_tokens, int) or not 0 <= max_tokens <= 2 ** 30:
+        raise ValueError("max_tokens must be an integer in [0, 2^30]")
     for name, t in (("page_counts", page_counts), ("seq_lens", seq_lens), ("new_lens", new_lens)):
         _ints(name, t, (b,))
     _ints("free_count", free_count, (1,))
@@ -200,7 +202,7 @@ def paged_append(k, v, k_cache, v_cache, slots, q=None, rotary_params=None, posi
         raise ValueError(f"Feature dimension must be even, got {dim}")
     if rotary_params is None and (q is not None or positions is not None or sections is not None):
         raise ValueError("q, positions and sections go with rotary_params")
-    _no_gradient("paged_append", k, v, q)
+    _no_gradient("paged_append", k, v, q, k_cache, v_cache)
     dev = _one_device(k_cache, v_cache, k, v, q, slots)
     axes = axis_arguments(rotary_params, positions, sections, dim, (tokens,), dev) if rotary_params is not None \
         else None
@@ -341,6 +343,7 @@ def paged_commit(k_cache, v_cache, block_table, base_lens, seq_lens, accepted) -
     _ints("accepted", accepted, (b, path))
     if path > 256:
         raise ValueError("an accepted path may have at most 256 tokens")
+    _no_gradient("paged_commit", k_cache, v_cache)
     dev = _one_device(k_cache, v_cache, block_table, base_lens, seq_lens, accepted)
     block_table, accepted = _rows(block_table), _rows(accepted)
     base_lens, seq_lens = base_lens.contiguous(), seq_lens.contiguous()

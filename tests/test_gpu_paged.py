@@ -433,6 +433,53 @@ def test_attention_pieces_of_every_length(dim, new, group):
         assert orc.rel_err(host(outs[0][i * new:(i + 1) * new]), host(one)) <= 2.0 ** -7
 
 
+@pytest.mark.parametrize("dim,group", [(64, 4), (128, 4), (128, 7), (128, 1)])
+def test_attention_mixed_batch(dim, group):
+    """Single tokens, trees and chunks in one batch: units of one and two query tiles follow each other in a CTA,
+    also where a share begins or ends inside one. Requests alone give the same up to the order of float32 sums."""
+    rng = np.random.default_rng(11)
+    new = rng.choice([1, 2, 7, 31, 33, 64, 65, 120, 300], 40)
+    lens = new + rng.integers(0, 900, 40)
+    b = Batch(12, new, lens, 2, group, dim, 32, BF)
+    args = b.args()
+    outs = [afa.afa_paged(*args) for _ in range(20)]
+    assert _lib.device_status(outs[0].device) == 0 and all(torch.equal(o, outs[0]) for o in outs)
+    q, k, v, table, slens, cu, _ = args
+    for i in range(0, 40, 3):
+        at = slice(int(b.cu[i]), int(b.cu[i + 1]))
+        one = afa.afa_paged(q[at], k, v, table[i:i + 1], slens[i:i + 1], i32([0, new[i]]))
+        # one rounding of the weights (2^-8 of three times the largest output) on each side and of the outputs
+        assert orc.rel_err(host(outs[0][at]), host(one)) <= 2 * 2.0 ** -8 * 4
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_offsets_past_32_bits(new):
+    """Pages of a cache of more than 2^31 elements, through append, attention and commit."""
+    pages, kv, page, dim = 140000, 1, 128, 128
+    k_cache, v_cache = (torch.empty((pages, kv, page, dim), dtype=BF, device="cuda") for _ in range(2))
+    assert k_cache.numel() > 2 ** 31
+    far, near = pages - 1, 5
+    for x in (k_cache, v_cache):
+        x[[far, near]] = torch.randn((2, kv, page, dim), device="cuda").to(BF)
+    table, n = np.array([[far, near]]), new
+    small = [torch.stack([x[far], x[near]]) for x in (k_cache, v_cache)]
+    q, k, v = (torch.randn((n, h, dim), device="cuda").to(BF) for h in (4, kv, kv))
+    length = 160 if n == 1 else 220
+    pos = np.arange(length - n, length)
+    slots = np.where(pos < page, far, near) * page + pos % page
+    assert afa.paged_append(k, v, k_cache, v_cache, dev(slots)) is None
+    assert afa.paged_append(k, v, *small, dev(np.where(pos < page, 0, 1) * page + pos % page)) is None
+    args = (i32([length]), i32([0, n]))
+    got = afa.afa_paged(q, k_cache, v_cache, i32(table), *args)
+    assert torch.equal(got, afa.afa_paged(q, *small, i32([[0, 1]]), *args))
+    accepted = i32([[1, 30, 39]])
+    base, lens = i32([100]), i32([length])
+    assert torch.equal(afa.paged_commit(k_cache, v_cache, i32(table), base, lens, accepted),
+                       afa.paged_commit(*small, i32([[0, 1]]), base, lens, accepted))
+    for x, y in zip((k_cache, v_cache), small):
+        assert torch.equal(x[far], y[0]) and torch.equal(x[near], y[1])
+
+
 def test_step_captured_and_replayed_with_other_lengths():
     """Plan, append and attention in one graph: the lengths it was captured with do not matter."""
     rng = np.random.default_rng(8)

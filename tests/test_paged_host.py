@@ -34,6 +34,7 @@ def _plan(**change):
     ({"page_size": 8}, ValueError),
     ({"page_size": 512}, ValueError),
     ({"max_tokens": -1}, ValueError),
+    ({"max_tokens": 2 ** 30 + 1}, ValueError),
     ({"parents": _z(2, 257)}, ValueError),
     ({"parents": _z(3, 4)}, ValueError),
     ({}, ValueError),  # CPU tensors
@@ -93,6 +94,8 @@ def _append(**change):
     ({"q": _z(3, 4, 8, dtype=torch.float32)}, ValueError),  # q without tables
     ({"q": _z(4, 4, 8, dtype=torch.float32)}, ValueError),
     ({"positions": _z(1, 3)}, ValueError),
+    ({"k": _z(3, 2, 8, dtype=torch.float32).requires_grad_(True)}, ValueError),
+    ({"k_cache": _z(5, 2, 16, 8, dtype=torch.float32).requires_grad_(True)}, ValueError),
     ({}, ValueError),  # CPU tensors
 ])
 def test_append_refusals(change, error):
@@ -113,6 +116,7 @@ def _commit(**change):
     ({"accepted": _z(2, 4, dtype=torch.int64)}, TypeError),
     ({"base_lens": _z(3)}, ValueError),
     ({"block_table": _z(6)}, ValueError),
+    ({"v_cache": _z(5, 2, 16, 8, dtype=torch.float32).requires_grad_(True)}, ValueError),
     ({"v_cache": _z(5, 2, 16, 6, dtype=torch.float32)}, ValueError),
     ({}, ValueError),  # CPU tensors
 ])
