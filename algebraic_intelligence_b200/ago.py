@@ -21,6 +21,7 @@ the rotations as one pass over q and k.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import NamedTuple, Optional
 
 import numpy as np
@@ -173,26 +174,33 @@ class AxisArguments(NamedTuple):
     sections: ctypes.Array
 
 
+@functools.lru_cache(maxsize=1024)
+def _sections(sections, pairs):
+    """Channel pairs of each axis, checked, as a C array."""
+    if not 1 <= len(sections) <= 4:
+        raise ValueError("between one and four position axes are supported")
+    if min(sections) < 0 or sum(sections) > pairs:
+        raise ValueError(f"sections must be nonnegative and sum to at most {pairs}, got {sections}")
+    return _lib.ints(*map(int, sections))
+
+
 def axis_arguments(rotary_params, positions, sections, dim, shape, device) -> AxisArguments:
     """Tables, positions (axes, *shape) and channel pairs per axis of a rotation, checked, and on ``device`` if one
     is given."""
     if positions is None or sections is None:
         raise ValueError("a rotation needs positions and sections")
-    sections = tuple(map(int, sections))
     pairs = dim // 2
-    if not 1 <= len(sections) <= 4:
-        raise ValueError("between one and four position axes are supported")
-    if min(sections) < 0 or sum(sections) > pairs:
-        raise ValueError(f"sections must be nonnegative and sum to at most {pairs}, got {sections}")
+    sections = _sections(tuple(sections), pairs)
     c, s = _extract_cs(rotary_params)
     if isinstance(c, np.ndarray):
         c = torch.from_numpy(np.ascontiguousarray(c))
     if isinstance(s, np.ndarray):
         s = torch.from_numpy(np.ascontiguousarray(s))
     if not isinstance(c, torch.Tensor) or not isinstance(s, torch.Tensor) or c.dtype not in _TABLE_DTYPES \
-            or s.dtype != c.dtype:
+            or s.dtype is not c.dtype:
         raise TypeError("the rotary tables must share a dtype: float32, bfloat16 or float64")
-    if c.shape != s.shape or c.ndim == 0 or c.shape[-1] != pairs or c.numel() == 0:
+    rows = c.shape
+    if rows != s.shape or len(rows) == 0 or rows[-1] != pairs or c.numel() == 0:
         raise ValueError(f"rotary tables must have shape (positions, {pairs}), got {tuple(c.shape)} and "
                          f"{tuple(s.shape)}")
     if c.requires_grad or s.requires_grad:
@@ -200,18 +208,21 @@ def axis_arguments(rotary_params, positions, sections, dim, shape, device) -> Ax
     p = positions if isinstance(positions, torch.Tensor) else torch.as_tensor(np.asarray(positions))
     if p.dtype != torch.int32 and p.dtype != torch.int64:
         raise TypeError("positions must be int32 or int64")
-    if p.shape != (len(sections), *shape):
-        raise ValueError(f"positions must have shape {(len(sections), *shape)}, got {tuple(p.shape)}")
+    axes = len(sections)
+    if p.shape != (axes, *shape):
+        raise ValueError(f"positions must have shape {(axes, *shape)}, got {tuple(p.shape)}")
     length = c.numel() // pairs
-    if not p.is_cuda and p.numel() and not (0 <= int(p.min()) and int(p.max()) < length):
+    if device is None and not p.is_cuda and p.numel() and not (0 <= int(p.min()) and int(p.max()) < length):
         raise ValueError(f"positions must lie in [0, {length}), the tables' rows")
     if device is not None and not c.device == s.device == p.device == device:
+        if not p.is_cuda and p.numel() and not (0 <= int(p.min()) and int(p.max()) < length):
+            raise ValueError(f"positions must lie in [0, {length}), the tables' rows")
         if any(x.is_cuda and x.device != device for x in (c, s, p)):
             raise ValueError(f"tables and positions must be on {device}")
         c, s, p = c.to(device), s.to(device), p.to(device)
     if c.ndim != 2:
         c, s = c.reshape(length, pairs), s.reshape(length, pairs)
-    return AxisArguments(c.contiguous(), s.contiguous(), p, _lib.ints(*sections))
+    return AxisArguments(c.contiguous(), s.contiguous(), p, sections)
 
 
 def _row_strides(t, token_major):

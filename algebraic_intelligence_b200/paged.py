@@ -34,6 +34,9 @@ from .ago import axis_arguments
 __all__ = ["PagedPlan", "paged_plan", "paged_append", "afa_paged", "paged_commit", "paged_workspace_bytes"]
 
 
+_I32 = torch.int32
+
+
 class PagedPlan(NamedTuple):
     """What ``paged_plan`` returns (T = max_tokens, B requests)."""
     slots: torch.Tensor        # (T,) int64: cache row page * page_size + offset, -1 behind the last token
@@ -53,7 +56,7 @@ def _check_page_size(page_size) -> None:
 
 
 def _ints(name, t, shape):
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+    if not isinstance(t, torch.Tensor) or t.dtype is not _I32:
         raise TypeError(f"{name} must be an int32 tensor")
     if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
@@ -134,8 +137,10 @@ def paged_plan(block_table, page_counts, seq_lens, new_lens, free_pages, free_co
     _check_page_size(page_size)
     if not isinstance(max_tokens, int) or not 0 <= max_tokens <= 2 ** 30:
         raise ValueError("max_tokens must be an integer in [0, 2^30]")
-    for name, t in (("page_counts", page_counts), ("seq_lens", seq_lens), ("new_lens", new_lens)):
-        _ints(name, t, (b,))
+    shape = (b,)
+    _ints("page_counts", page_counts, shape)
+    _ints("seq_lens", seq_lens, shape)
+    _ints("new_lens", new_lens, shape)
     _ints("free_count", free_count, (1,))
     if not isinstance(free_pages, torch.Tensor) or free_pages.dtype != torch.int32:
         raise TypeError("free_pages must be an int32 tensor")
@@ -153,19 +158,20 @@ def paged_plan(block_table, page_counts, seq_lens, new_lens, free_pages, free_co
     page_counts, seq_lens, new_lens = page_counts.contiguous(), seq_lens.contiguous(), new_lens.contiguous()
     parents = parents.contiguous() if parents is not None else None
     # One allocation, cut up: int64 slots first, then 32-bit words.
-    words = (nodes + 31) // 32
-    sizes = (2 * max_tokens, max_tokens, max_tokens, b + 1, b, b, 1, max_tokens * words, (b + 3) // 4)
-    buf = torch.empty(sum(sizes), dtype=torch.int32, device=dev)
-    slots, rows, positions, cu, lens_out, held_out, free_out, ancestors, granted = buf.split_with_sizes(sizes)
-    base, at = buf.data_ptr(), [0]
-    for n in sizes:
-        at.append(at[-1] + 4 * n)
+    words, t = (nodes + 31) // 32, max_tokens
+    w, g = t * words, (b + 3) // 4
+    buf = torch.empty(4 * t + 3 * b + 2 + w + g, dtype=torch.int32, device=dev)
+    slots, rows, positions, cu, lens_out, held_out, free_out, ancestors, granted = buf.split_with_sizes(
+        (2 * t, t, t, b + 1, b, b, 1, w, g))
+    per_request = buf.data_ptr() + 16 * t  # cu_tokens
+    behind = per_request + 12 * b + 8      # ancestors
     rc = _lib.call(
         dev, _lib.load().afa_paged_plan, block_table.data_ptr(), page_counts.data_ptr(), seq_lens.data_ptr(),
         new_lens.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), parents.data_ptr() if nodes else None,
-        *(base + x for x in at[:7]), base + at[8], base + at[7], b, cols, page_size, free_pages.shape[0], max_tokens,
-        nodes)
-    _lib.check(rc, "afa_paged_plan")
+        per_request - 16 * t, per_request - 8 * t, per_request - 4 * t, per_request, per_request + 4 * b + 4,
+        per_request + 8 * b + 4, behind - 4, behind + 4 * w, behind, b, cols, page_size, free_pages.shape[0], t, nodes)
+    if rc:
+        _lib.check(rc, "afa_paged_plan")
     return PagedPlan(slots.view(torch.int64), rows, positions, cu, lens_out, held_out, free_out,
                      granted.view(torch.bool)[:b], ancestors.view(max_tokens, words) if nodes else None)
 
@@ -227,7 +233,8 @@ def paged_append(k, v, k_cache, v_cache, slots, q=None, rotary_params=None, posi
         None if q is None else _lib.longs(*q.stride()[:2]), None if out is None else out.data_ptr(),
         0 if q is None else q.shape[1], *pos, tokens, heads, dim, pages, page_size,
         _lib.dtype_code(k_cache.dtype))
-    _lib.check(rc, "afa_paged_append")
+    if rc:
+        _lib.check(rc, "afa_paged_append")
     return out
 
 
@@ -312,7 +319,8 @@ def afa_paged(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, ancestors=N
         seq_lens.data_ptr(), cu_tokens.data_ptr(), ancestors.data_ptr() if words else None,
         ancestors.stride(0) if words else 0, words, b, tokens, heads, kv_heads, dim, cols, page_size, pages, code,
         float(sink_omega), workspace.data_ptr(), need)
-    _lib.check(rc, "afa_paged")
+    if rc:
+        _lib.check(rc, "afa_paged")
     return (out, den) if return_denominator else out
 
 
@@ -355,5 +363,6 @@ def paged_commit(k_cache, v_cache, block_table, base_lens, seq_lens, accepted) -
         block_table.stride(0), base_lens.data_ptr(), seq_lens.data_ptr(), accepted.data_ptr(),
         accepted.stride(0) if path else 0, lens.data_ptr(), b, path, layers, heads, dim, cols, pages, page_size,
         _lib.dtype_code(k_cache.dtype))
-    _lib.check(rc, "afa_paged_commit")
+    if rc:
+        _lib.check(rc, "afa_paged_commit")
     return lens
