@@ -316,41 +316,57 @@ __global__ void __launch_bounds__(kCombineWarps * 32) paged_combine_kernel(const
   const int4 meta = *reinterpret_cast<const int4*>(a.meta + 4 * c);
   const int b = meta.y, h = meta.z, u = meta.w, D = a.D;
   if (b < 0) return;
-  int last = c + 1;
-  while (last < ctas - 1 && a.meta[4 * last] == 0) ++last;
+  const int lane = threadIdx.x & 31;
+  int last = c + 1;  // the CTA that ends the unit: 32 are looked at in one step
+  while (true) {
+    const unsigned ends = __ballot_sync(0xffffffffu, last + lane >= ctas - 1 || a.meta[4 * (last + lane)] != 0);
+    if (ends) {
+      last += __ffs(ends) - 1;
+      break;
+    }
+    last += 32;
+  }
   const PagedReq req = paged_req(a, b);
   const long long row0 = static_cast<long long>(u) * a.unit_rows;
   const int rows = static_cast<int>(min(static_cast<long long>(a.unit_rows), static_cast<long long>(req.n) * a.G - row0));
   const long long size = static_cast<long long>(a.frag_rows) * (D + 1);
-  const A* first = static_cast<const A*>(a.frag) + (2LL * c + 1) * size;
-  const A* rest = static_cast<const A*>(a.frag) + 2LL * (c + 1) * size;  // of CTA c + 1; 2 * size apart
-  const int nrest = last - c;
+  // Fragment x of the unit: CTA c's fragment 1, then the next CTAs' fragments 0.
+  const A* frag = static_cast<const A*>(a.frag) + 2LL * c * size;
+  const int n = last - c + 1;
   const A sink = sizeof(A) == 8 ? static_cast<A>(a.sink_d) : static_cast<A>(a.sink);
-  const int lane = threadIdx.x & 31;
   const long long den_at = static_cast<long long>(a.frag_rows) * D;
+  // Four fragments' loads are under way at once, whatever their number: with few
+  // query rows a latency for each CTA's entry and fragment was most of this
+  // kernel (one token against 4000 keys of 8 heads: 18.4 us together, now 15.6;
+  // against 65536: 59.4, now 55.1).
+  auto each = [&](auto&& load) {
+    for (int x0 = 0; x0 < n; x0 += 4)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int x = x0 + i;
+        load(frag + (x == 0 ? size : 2LL * x * size), x < n);
+      }
+  };
   for (int r = blockIdx.y * kCombineWarps + (threadIdx.x >> 5); r < rows; r += gridDim.y * kCombineWarps) {
-    A den = first[den_at + r];
-#pragma unroll 4
-    for (int x = 0; x < nrest; ++x) den += rest[2LL * x * size + den_at + r];
-    den += sink;
+    A den = sink;
+    each([&](const A* f, bool in) { den += in ? f[den_at + r] : A(0); });
     const long long row = row0 + r, tok = row / a.G;
     const long long orow = (req.tok0 + tok) * a.Hkv * a.G + static_cast<long long>(h) * a.G + (row - tok * a.G);
     T* out = static_cast<T*>(a.out) + orow * D;
     for (int col = lane * W; col < D; col += 32 * W) {
       const long long at = static_cast<long long>(r) * D + col;
-      A sum[W];
-      auto add = [&](const A* f, bool set) {
-        alignas(16) A v[W];
-        if constexpr (W * sizeof(A) == 16)
-          *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(f + at);
-        else
-          v[0] = f[at];
+      A sum[W] = {};
+      each([&](const A* f, bool in) {
+        alignas(16) A v[W] = {};
+        if (in) {
+          if constexpr (W * sizeof(A) == 16)
+            *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(f + at);
+          else
+            v[0] = f[at];
+        }
 #pragma unroll
-        for (int i = 0; i < W; ++i) sum[i] = set ? v[i] : sum[i] + v[i];
-      };
-      add(first, true);
-#pragma unroll 4
-      for (int x = 0; x < nrest; ++x) add(rest + 2LL * x * size, false);
+        for (int i = 0; i < W; ++i) sum[i] += v[i];
+      });
       alignas(16) T y[W];
 #pragma unroll
       for (int i = 0; i < W; ++i) y[i] = from_acc<T>(den > A(0) ? sum[i] / den : A(0));

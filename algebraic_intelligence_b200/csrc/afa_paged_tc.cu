@@ -628,7 +628,7 @@ cudaError_t launch_hd(const PagedArgs& a, int ctas, cudaStream_t stream, const c
 }  // namespace
 
 // TMA reads rows that start on 16 bytes at strides of 16 bytes; a stride of 0
-// (a broadcast view) or past 2^40 bytes is no tensor map's.
+// (a broadcast view) or of 2^31 elements or more is left to the CUDA cores.
 bool paged_tc_supported(const PagedArgs& a, int dtype) {
   if (dtype != kBF16 || (a.D != 64 && a.D != 128) || a.G > 128) return false;
   for (const void* p : {a.q, a.k, a.v})
