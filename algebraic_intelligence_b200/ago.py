@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import operator
 from typing import NamedTuple, Optional
 
 import numpy as np
@@ -181,7 +182,7 @@ def _sections(sections, pairs):
         raise ValueError("between one and four position axes are supported")
     if min(sections) < 0 or sum(sections) > pairs:
         raise ValueError(f"sections must be nonnegative and sum to at most {pairs}, got {sections}")
-    return _lib.ints(*map(int, sections))
+    return _lib.ints(*sections)
 
 
 def axis_arguments(rotary_params, positions, sections, dim, shape, device) -> AxisArguments:
@@ -190,7 +191,7 @@ def axis_arguments(rotary_params, positions, sections, dim, shape, device) -> Ax
     if positions is None or sections is None:
         raise ValueError("a rotation needs positions and sections")
     pairs = dim // 2
-    sections = _sections(tuple(sections), pairs)
+    sections = _sections(tuple(map(operator.index, sections)), pairs)
     c, s = _extract_cs(rotary_params)
     if isinstance(c, np.ndarray):
         c = torch.from_numpy(np.ascontiguousarray(c))

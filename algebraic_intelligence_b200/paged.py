@@ -94,6 +94,8 @@ def _caches(k_cache, v_cache, ndims=(4,)):
         raise TypeError("k_cache and v_cache must share a dtype")
     pages, heads, page_size, dim = shape[-4:]
     _check_page_size(page_size)
+    if 0 in shape:
+        raise ValueError(f"the caches must not be empty, got {tuple(shape)}")
     if k_cache.stride()[-1] != 1 or v_cache.stride()[-1] != 1:
         raise ValueError("a cache row's channels must be contiguous")
     return pages, heads, page_size, dim
@@ -227,8 +229,9 @@ def paged_append(k, v, k_cache, v_cache, slots, q=None, rotary_params=None, posi
     else:
         pos = (None, None, 0, 0, None, None, 0, None, 0)
     rc = _lib.call(
-        dev, _lib.load().afa_paged_append, k.data_ptr(), _lib.longs(*k.stride()[:2]), v.data_ptr(), _lib.longs(*v.stride()[:2]),
-        k_cache.data_ptr(), _lib.longs(*k_cache.stride()[:3]), v_cache.data_ptr(), _lib.longs(*v_cache.stride()[:3]),
+        dev, _lib.load().afa_paged_append, k.data_ptr(), _lib.longs(*k.stride()[:2]), v.data_ptr(),
+        _lib.longs(*v.stride()[:2]), k_cache.data_ptr(), _lib.longs(*k_cache.stride()[:3]), v_cache.data_ptr(),
+        _lib.longs(*v_cache.stride()[:3]),
         slots.data_ptr(), None if q is None else q.data_ptr(),
         None if q is None else _lib.longs(*q.stride()[:2]), None if out is None else out.data_ptr(),
         0 if q is None else q.shape[1], *pos, tokens, heads, dim, pages, page_size,
@@ -297,7 +300,7 @@ def afa_paged(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, ancestors=N
         ancestors = _rows(ancestors)
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous()):
         raise ValueError("out must be a contiguous tensor of q's shape and dtype")
-    _no_gradient("afa_paged", q, k_cache, v_cache)
+    _no_gradient("afa_paged", q, k_cache, v_cache, out)
     dev = _one_device(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, ancestors, out, workspace)
     q, block_table = _rows(q), _rows(block_table)
     seq_lens, cu_tokens = seq_lens.contiguous(), cu_tokens.contiguous()
@@ -359,8 +362,9 @@ def paged_commit(k_cache, v_cache, block_table, base_lens, seq_lens, accepted) -
     layers = k_cache.shape[0] if k_cache.ndim == 5 else 1
     strides = [(0, *t.stride()[:3]) if t.ndim == 4 else t.stride()[:4] for t in (k_cache, v_cache)]
     rc = _lib.call(
-        dev, _lib.load().afa_paged_commit, k_cache.data_ptr(), _lib.longs(*strides[0]), v_cache.data_ptr(), _lib.longs(*strides[1]), block_table.data_ptr(),
-        block_table.stride(0), base_lens.data_ptr(), seq_lens.data_ptr(), accepted.data_ptr(),
+        dev, _lib.load().afa_paged_commit, k_cache.data_ptr(), _lib.longs(*strides[0]), v_cache.data_ptr(),
+        _lib.longs(*strides[1]), block_table.data_ptr(), block_table.stride(0), base_lens.data_ptr(),
+        seq_lens.data_ptr(), accepted.data_ptr(),
         accepted.stride(0) if path else 0, lens.data_ptr(), b, path, layers, heads, dim, cols, pages, page_size,
         _lib.dtype_code(k_cache.dtype))
     if rc:

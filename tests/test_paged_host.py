@@ -7,6 +7,7 @@ import torch
 
 import algebraic_intelligence_b200 as afa
 from algebraic_intelligence_b200 import _lib
+from algebraic_intelligence_b200.ago import axis_arguments
 from oracle import paged_oracle as po
 
 I32 = torch.int32
@@ -156,6 +157,31 @@ def _rotate(**change):
 def test_rotation_refusals(change, error):
     with pytest.raises(error):
         _rotate(**change)
+
+
+@pytest.mark.parametrize("shape", [(0, 2, 16, 64), (5, 0, 16, 64), (5, 2, 16, 0)])
+def test_empty_caches_are_refused(shape):
+    empty = dict(k_cache=torch.zeros(shape), v_cache=torch.zeros(shape))
+    for call in (_attend, _append, _commit):
+        with pytest.raises(ValueError, match="must not be empty"):
+            call(**empty)
+
+
+def test_out_that_wants_a_gradient_is_refused():
+    with pytest.raises(ValueError, match="has no gradient"):
+        _attend(out=_z(3, 4, 64, dtype=torch.bfloat16).requires_grad_(True))
+
+
+def test_sections_are_integers():
+    with pytest.raises(TypeError):
+        _rotate(sections=(2.5, 1))
+    # Read at every call, whatever holds them.
+    sections = [torch.tensor(2), torch.tensor(1)]
+    assert np.array_equal(axis_arguments((np.ones((9, 4)), np.zeros((9, 4))), np.zeros((2, 5), np.int32), sections, 8,
+                                         (5,), None).sections[:2], [2, 1])
+    sections[0].add_(1)
+    assert np.array_equal(axis_arguments((np.ones((9, 4)), np.zeros((9, 4))), np.zeros((2, 5), np.int32), sections, 8,
+                                         (5,), None).sections[:2], [3, 1])
 
 
 def test_c_entries_refuse_before_any_cuda_call():
