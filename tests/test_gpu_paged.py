@@ -322,6 +322,9 @@ CASES = {
     "wide-chunk": dict(new=[300], lens=[513], kv=1, group=2, page=256),
     "tree": dict(new=[20, 1, 40, 7], lens=[20, 260, 333, 135], kv=2, group=4, page=16, tree=True),
     "wide-tree": dict(new=[65, 129], lens=[190, 400], kv=1, group=5, page=64, tree=True),
+    # units cut into fragments of more than 32 CTAs
+    "one-long": dict(new=[1], lens=[30011], kv=1, group=3, page=128),
+    "long-tree": dict(new=[70], lens=[9000], kv=1, group=2, page=32, tree=True),
     "empty-requests": dict(new=[0, 2, 0, 0, 3, 0], lens=[50, 2, 0, 7, 64, 0], kv=2, group=2, page=16),
     "many-rows-per-head": dict(new=[2, 5], lens=[140, 70], kv=1, group=64, page=16),
 }
