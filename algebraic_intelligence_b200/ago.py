@@ -255,6 +255,14 @@ def _rotate_axes(q, k, axes: AxisArguments, backward: bool):
     return qo, ko
 
 
+def _on_pairs(t):
+    """t, or a copy where a row starts off a channel pair's alignment (the gradient of a concatenation's part does)."""
+    if t is None or t.stride(-1) != 1 or (t.data_ptr() % (2 * t.element_size()) == 0 and
+                                          not any(s & 1 for s in t.stride()[:-1])):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 class _RotateAxes(torch.autograd.Function):
     """A rotation's gradient is the rotation the other way, which is differentiable again."""
 
@@ -268,6 +276,7 @@ class _RotateAxes(torch.autograd.Function):
     @staticmethod
     def backward(ctx, gq, gk=None):
         c, s, positions = ctx.saved_tensors
+        gq, gk = _on_pairs(gq), _on_pairs(gk)
         if torch.is_grad_enabled():  # a gradient of the gradient may follow
             g = _RotateAxes.apply(gq, gk, c, s, positions, ctx.sections, not ctx.turn_back)
             g = (g, None) if gk is None else g
@@ -289,8 +298,10 @@ def apply_ago_rotations_axes(q, k, rotary_params, positions, sections):
     NaN on the device. ``rotary_params`` as in ``apply_ago_rotations``, (positions,
     dim / 2). Unlike there the tables keep their dtype: the arithmetic is
     float32 (float64 for float64 inputs) with one rounding, which a bfloat16
-    table would limit to 2^-9. Differentiable in q and k. Returns contiguous
-    (q_rot, k_rot).
+    table would limit to 2^-9. Differentiable in q and k (before a backward pass
+    is captured into a CUDA graph, release what was computed from the same
+    leaves outside of it: PyTorch would wait for those leaves' stream). Returns
+    contiguous (q_rot, k_rot).
     """
     if q.ndim not in (3, 4):
         raise ValueError(f"q must have shape (batch, heads, tokens, dim) or (tokens, heads, dim), got {tuple(q.shape)}")

@@ -217,6 +217,46 @@ def test_rotation_gradient_against_differences():
     assert not q.grad.any()
 
 
+def test_rotation_gradient_that_starts_off_a_pair():
+    """The gradient of a part of a concatenation is a view whose rows may start anywhere."""
+    rng = np.random.default_rng(6)
+    c, s = tables(32, 16, F32)
+    q = dev(rng.standard_normal((5, 3, 32)), BF).requires_grad_(True)
+    pos, up = dev(rng.integers(0, 16, (1, 5))), dev(rng.standard_normal((5, 3, 33)), BF)
+    first = torch.zeros(5, 3, 1, dtype=BF, device="cuda")
+    qr, _ = afa.apply_ago_rotations_axes(q, None, (c, s), pos, (16,))
+    got, = torch.autograd.grad(torch.cat((first, qr), -1), q, up)
+    qr, _ = afa.apply_ago_rotations_axes(q, None, (c, s), pos, (16,))
+    want, = torch.autograd.grad(qr, q, up[..., 1:].contiguous())
+    assert torch.equal(got, want)
+
+
+def test_rotation_and_gradient_captured():
+    rng = np.random.default_rng(7)
+    c, s = tables(64, 32, F32)
+    x = [dev(rng.standard_normal((1, h, 11, 64)), BF) for h in (4, 2, 4, 2)]
+    pos = dev(rng.integers(0, 32, (3, 1, 11)))
+
+    def step():
+        q, k = (t.detach().requires_grad_(True) for t in x[:2])
+        qr, kr = afa.apply_ago_rotations_axes(q, k, (c, s), pos, (12, 8, 12))
+        return (qr.detach(), kr.detach(), *torch.autograd.grad((qr, kr), (q, k), x[2:]))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for t in x:
+        t.copy_(dev(rng.standard_normal(t.shape), BF))
+    pos.copy_(dev(rng.integers(0, 32, (3, 1, 11))))
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
 # ---------------------------------------------------------------------------------------------------------
 # paged_append
 # ---------------------------------------------------------------------------------------------------------
