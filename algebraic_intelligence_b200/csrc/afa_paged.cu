@@ -123,8 +123,8 @@ __global__ void __launch_bounds__(kSimtThreads) afa_paged_simt_kernel(const __gr
   };
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // see paged_combine_kernel
-  PagedWalk walk;
-  walk.init(a, paged_share<kSimtThreads>(a, share_sm));
+  PagedWalk<false> walk;
+  walk.init(a, paged_share<kSimtThreads, false>(a, share_sm));
   if (tid == 0) paged_meta_clear(a.meta);
   PagedPiece p;
   while (walk.next(a, p)) {
@@ -581,7 +581,8 @@ extern "C" int afa_paged(const void* q, const long long* q_strides, const void* 
   const bool tc = paged_tc_supported(a, dtype);
   const int nt = tc ? paged_tr_rows(batch, tokens, a.G) : 0;
   a.unit_rows = nt ? nt / a.G * a.G : tc ? paged_tc_unit_rows(a.G) : simt_unit_rows(batch, tokens, a.G);
-  a.min_share = tc ? 2 : 1;
+  // Tensor cores: two key tiles at least (of a pair of query tiles, if most units are pairs).
+  a.min_share = !tc ? 1 : nt || static_cast<long long>(tokens) * a.G / batch <= a.unit_rows / 2 ? 2 : 4;
   if (!tc) {
     const size_t es = dtype_size(dtype), run = es * (dtype == kF64 ? 2 : 4);  // a channel group in memory
     a.wide = static_cast<size_t>(D) * es % run == 0;

@@ -3,10 +3,11 @@
 // A work unit is up to unit_rows query rows (row r of a request: token r / G,
 // query head r % G of the key head's group) of one request and key head against
 // the keys those rows can see, in tiles of kPagedTile. The units, ordered by
-// request, key head and rows, are laid end to end, one cost unit per key tile,
-// and CTA c takes the c-th of equal shares of that line: every CTA reads the
-// same number of key tiles whatever the lengths are, without knowing them on
-// the host. A unit cut by the end of a share is computed in fragments. Octic
+// request, key head and rows, are laid end to end, one cost unit per key tile
+// (two where a unit has two query tiles), and CTA c takes the c-th of equal
+// shares of that line, the key tiles that begin in it: every CTA has about the
+// same work whatever the lengths are, without knowing them on the host. A unit
+// cut by the end of a share is computed in fragments. Octic
 // weights need no running maximum, so fragments only add; they go to a
 // workspace and paged_combine_kernel adds them in CTA order (no atomics: the
 // same inputs give the same bits) and divides.
@@ -48,19 +49,31 @@ __device__ __forceinline__ int paged_tiles(const PagedArgs& a, const PagedReq& r
   return (paged_visible(a, r, (u + 1) * a.unit_rows) + kPagedTile - 1) / kPagedTile;
 }
 
-// Cost of a unit: its key tiles; a unit that sees no key still writes its rows.
+// log2 of a key tile's cost. PAIRS: a unit with two query tiles takes 1.6 to 1.8
+// times as long for a key tile as one with a single one, and counts twice (counted
+// alike, the CTAs with pairs ended last: 16 trees of 17 to 34 nodes over 6000 keys
+// took 104 us, 88 now, of 24 to 48 nodes 120, 113 now).
+template <bool PAIRS>
+__device__ __forceinline__ int paged_tile_shift(const PagedArgs& a, const PagedReq& r, int u) {
+  return PAIRS && r.n * a.G - u * a.unit_rows > a.unit_rows / 2;
+}
+
+// Cost of a unit: its key tiles'; a unit that sees no key still writes its rows.
+template <bool PAIRS>
 __device__ __forceinline__ int paged_cost(const PagedArgs& a, const PagedReq& r, int u) {
   const int t = paged_tiles(a, r, u);
-  return t > 0 ? t : 1;
+  return (t > 0 ? t : 1) << paged_tile_shift<PAIRS>(a, r, u);
 }
 
 // Cost of a request's units for one key head.
+template <bool PAIRS>
 __device__ __forceinline__ long long paged_req_cost(const PagedArgs& a, const PagedReq& r) {
   const int units = paged_units(a, r);
   if (units == 0) return 0;
-  if (a.anc) return static_cast<long long>(units) * paged_cost(a, r, 0);
+  if (a.anc)  // all but the last are alike
+    return static_cast<long long>(units - 1) * paged_cost<PAIRS>(a, r, 0) + paged_cost<PAIRS>(a, r, units - 1);
   long long c = 0;
-  for (int u = 0; u < units; ++u) c += paged_cost(a, r, u);
+  for (int u = 0; u < units; ++u) c += paged_cost<PAIRS>(a, r, u);
   return c;
 }
 
@@ -74,7 +87,7 @@ struct PagedShare {
 // This CTA's share. Called by all NT threads; `sm` is scratch of NT / 32 + 4
 // 8-byte words. Every CTA adds up the requests' costs by itself: it costs less
 // than a launch that would do it once.
-template <int NT>
+template <int NT, bool PAIRS>
 __device__ __forceinline__ PagedShare paged_share(const PagedArgs& a, long long* sm) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr int NW = NT / 32;
@@ -82,7 +95,7 @@ __device__ __forceinline__ PagedShare paged_share(const PagedArgs& a, long long*
   const int per = (a.B + NT - 1) / NT;
   const int b0 = min(static_cast<int>(threadIdx.x) * per, a.B), b1 = min(b0 + per, a.B);
   long long mine = 0;
-  for (int b = b0; b < b1; ++b) mine += paged_req_cost(a, paged_req(a, b)) * a.Hkv;
+  for (int b = b0; b < b1; ++b) mine += paged_req_cost<PAIRS>(a, paged_req(a, b)) * a.Hkv;
   long long inc = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -100,7 +113,8 @@ __device__ __forceinline__ PagedShare paged_share(const PagedArgs& a, long long*
   }
   const long long first = before + inc - mine;  // cost before this thread's requests
   PagedShare s;
-  const long long most = (total + a.min_share - 1) / a.min_share;
+  // PAIRS: no share is shorter than two, so that some key tile begins in each.
+  const long long most = PAIRS ? max(total / a.min_share, min(total, 1LL)) : (total + a.min_share - 1) / a.min_share;
   s.ctas = most < gridDim.x ? static_cast<int>(most) : static_cast<int>(gridDim.x);
   const int c = blockIdx.x;
   if (c >= s.ctas) {
@@ -114,7 +128,7 @@ __device__ __forceinline__ PagedShare paged_share(const PagedArgs& a, long long*
     long long x = lo - first;
     int b = b0;
     while (b < b1 - 1) {
-      const long long cost = paged_req_cost(a, paged_req(a, b)) * a.Hkv;
+      const long long cost = paged_req_cost<PAIRS>(a, paged_req(a, b)) * a.Hkv;
       if (x < cost) break;
       x -= cost;
       ++b;
@@ -137,8 +151,9 @@ struct PagedPiece {
   __device__ bool whole() const { return t0 == 0 && t1 == cost; }
 };
 
+template <bool PAIRS>
 struct PagedWalk {
-  int b, h, u, t, units;
+  int b, h, u, x, units;  // x: cost of unit u before the share
   long long left;
   PagedReq r;
 
@@ -147,55 +162,58 @@ struct PagedWalk {
     b = s.b;
     h = 0;
     u = 0;
-    t = 0;
+    x = 0;
     units = 0;
     if (left <= 0) return;
     r = paged_req(a, b);
     units = paged_units(a, r);
-    const long long cost = paged_req_cost(a, r);
+    const long long cost = paged_req_cost<PAIRS>(a, r);
     h = static_cast<int>(s.x / cost);
-    long long x = s.x - h * cost;
+    long long y = s.x - h * cost;
     if (a.anc) {
-      const int c = paged_cost(a, r, 0);
-      u = static_cast<int>(x / c);
-      x -= static_cast<long long>(u) * c;
+      const int c = paged_cost<PAIRS>(a, r, 0);
+      u = static_cast<int>(min(y / c, static_cast<long long>(units - 1)));
+      y -= static_cast<long long>(u) * c;
     } else {
       while (true) {
-        const int c = paged_cost(a, r, u);
-        if (x < c) break;
-        x -= c;
+        const int c = paged_cost<PAIRS>(a, r, u);
+        if (y < c) break;
+        y -= c;
         ++u;
       }
     }
-    t = static_cast<int>(x);
+    x = static_cast<int>(y);
   }
 
   __device__ __forceinline__ bool next(const PagedArgs& a, PagedPiece& p) {
-    if (left <= 0) return false;
-    if (u == units) {
-      u = 0;
-      if (++h == a.Hkv) {
-        h = 0;
-        do {
-          if (++b >= a.B) return false;
-          r = paged_req(a, b);
-          units = paged_units(a, r);
-        } while (units == 0);
+    while (left > 0) {
+      if (u == units) {
+        u = 0;
+        if (++h == a.Hkv) {
+          h = 0;
+          do {
+            if (++b >= a.B) return false;
+            r = paged_req(a, b);
+            units = paged_units(a, r);
+          } while (units == 0);
+        }
       }
+      p.b = b;
+      p.h = h;
+      p.u = u;
+      p.r = r;
+      p.tiles = paged_tiles(a, r, u);
+      p.cost = p.tiles > 0 ? p.tiles : 1;
+      const int sh = paged_tile_shift<PAIRS>(a, r, u), total = p.cost << sh;
+      const int end = left < total - x ? x + static_cast<int>(left) : total;
+      p.t0 = (x + sh) >> sh;  // the tiles that begin in [x, end)
+      p.t1 = (end + sh) >> sh;
+      left -= end - x;
+      x = 0;
+      ++u;
+      if (!PAIRS || p.t1 > p.t0) return true;
     }
-    p.b = b;
-    p.h = h;
-    p.u = u;
-    p.r = r;
-    p.tiles = paged_tiles(a, r, u);
-    p.cost = p.tiles > 0 ? p.tiles : 1;
-    p.t0 = t;
-    const long long end = t + left;
-    p.t1 = end < p.cost ? static_cast<int>(end) : p.cost;
-    left -= p.t1 - p.t0;
-    t = 0;
-    ++u;
-    return true;
+    return false;
   }
 };
 

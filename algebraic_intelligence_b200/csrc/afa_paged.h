@@ -25,7 +25,7 @@ struct PagedArgs {
   int B, T, Hkv, G, D, table_cols, page_shift, num_pages, words;
   int unit_rows;            // query rows (token, head of the group) per work unit
   int frag_rows;            // rows of a fragment: unit_rows, or all rows there can be if fewer
-  int min_share;            // key tiles of a CTA below which fewer CTAs run
+  int min_share;            // cost of a CTA's share below which fewer CTAs run
   int wide;                 // CUDA cores: rows can be read a channel group at a time
   double scale_d, sink_d;
   float scale, sink;

@@ -203,8 +203,8 @@ __global__ void __launch_bounds__(608, 1)
   }
   tc_fence_before();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // see paged_combine_kernel
-  PagedWalk walk;
-  walk.init(a, paged_share<C::kThreads>(a, reinterpret_cast<long long*>(smem + C::SHARE_OFF)));
+  PagedWalk<true> walk;
+  walk.init(a, paged_share<C::kThreads, true>(a, reinterpret_cast<long long*>(smem + C::SHARE_OFF)));
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;

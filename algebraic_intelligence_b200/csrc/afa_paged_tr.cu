@@ -208,8 +208,8 @@ __global__ void __launch_bounds__(608, 1)
   }
   tc_fence_before();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // see paged_combine_kernel
-  PagedWalk walk;
-  walk.init(a, paged_share<C::kThreads>(a, reinterpret_cast<long long*>(smem + C::SHARE_OFF)));
+  PagedWalk<false> walk;
+  walk.init(a, paged_share<C::kThreads, false>(a, reinterpret_cast<long long*>(smem + C::SHARE_OFF)));
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(608, 1)
     };
     // The tiles of all pieces are one stream: the scores run two tiles ahead of
     // the outputs, also from one piece into the next, with a walk of their own.
-    PagedWalk swalk = walk;
+    PagedWalk<false> swalk = walk;
     typename C::KPos kpos;
     typename C::VPos vpos;
     bool ok = true, s_more = true;
