@@ -590,6 +590,7 @@ extern "C" int afa_paged(const void* q, const long long* q_strides, const void* 
     for (long long s : {a.q_st, a.q_sh, a.k_sp, a.k_sh, a.k_sr, a.v_sp, a.v_sh, a.v_sr})
       a.wide = a.wide && s * static_cast<long long>(es) % static_cast<long long>(run) == 0;
   }
+  a.out_wide = reinterpret_cast<uintptr_t>(out) % 16 == 0;
   a.frag_rows = frag_rows_of(a.unit_rows, tokens, a.G);
   const char* detail = "";
   cudaError_t e;

@@ -27,6 +27,7 @@ struct PagedArgs {
   int frag_rows;            // rows of a fragment: unit_rows, or all rows there can be if fewer
   int min_share;            // cost of a CTA's share below which fewer CTAs run
   int wide;                 // CUDA cores: rows can be read a channel group at a time
+  int out_wide;             // out starts on 16 bytes
   double scale_d, sink_d;
   float scale, sink;
   int* meta;                // workspace: 4 ints per CTA (see PagedPiece)

@@ -562,9 +562,20 @@ __global__ void __launch_bounds__(608, 1)
             for (int kr = 0; kr < NCH; ++kr) {
               const int src = (lane & ~(NCH - 1)) + kr;
               const long long r = __shfl_sync(0xffffffffu, orow, src);
-              if (sub * 32 + src < live_rows)
-                *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + r * HD + col0 + 8 * gi) =
-                    make_uint4(pk[4 * kr], pk[4 * kr + 1], pk[4 * kr + 2], pk[4 * kr + 3]);
+              if (sub * 32 + src < live_rows) {
+                __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + r * HD + col0 + 8 * gi;
+                if (a.out_wide) {
+                  *reinterpret_cast<uint4*>(dst) =
+                      make_uint4(pk[4 * kr], pk[4 * kr + 1], pk[4 * kr + 2], pk[4 * kr + 3]);
+                } else {  // `out` may be any part of a larger buffer
+                  uint16_t* h = reinterpret_cast<uint16_t*>(dst);
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    h[2 * e] = static_cast<uint16_t>(pk[4 * kr + e]);
+                    h[2 * e + 1] = static_cast<uint16_t>(pk[4 * kr + e] >> 16);
+                  }
+                }
+              }
             }
           } else {
             // Eight lanes: 128 contiguous bytes of each of 4 rows.

@@ -326,7 +326,7 @@ AFA_API int afa_decode_noalloc(const void* q, const void* k_cache, const void* v
  *                 words is set. Keys whose table entry names no page of the
  *                 cache are not seen. Query heads [h q_heads / kv_heads, ...)
  *                 share key head h. out (tokens, q_heads, D) and d_total
- *                 (tokens, q_heads; may be NULL) are contiguous; a row that
+ *                 (tokens, q_heads; may be NULL) are contiguous, on any element; a row that
  *                 sees no key gives 0 and sink_omega, rows of no request are
  *                 not written. Cached rows of a request must be finite; what
  *                 lies behind its last token does not matter.

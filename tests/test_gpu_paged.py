@@ -679,3 +679,20 @@ def test_serving_with_drafted_trees(dtype, dim, page):
         owned = [int(table[b, j]) for b in range(batch) for j in range(int(held[b]))] + host(stack)[:int(free)].tolist()
         assert sorted(owned) == list(range(pool))
     assert _lib.device_status(out.device) == 0
+
+
+# ---------------------------------------------------------------------------------------------------------
+# Views, neighbours and values that the tests above do not have
+# ---------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,dim", [(BF, 128), (BF, 64), (BF, 96), (F32, 64), (F64, 64)])
+@pytest.mark.parametrize("name", ["decode", "chunk", "wide-chunk", "tree", "wide-tree", "long-tree"])
+def test_attention_out_that_starts_anywhere(name, dtype, dim):
+    """A contiguous part of a larger buffer, on any element: the bits of an output of its own, and nothing beside it."""
+    b = Batch(13, dim=dim, dtype=dtype, **CASES[name])
+    want = afa.afa_paged(*b.args())
+    for first in (1, 2, 4, 8, 11):
+        buf = torch.full((want.numel() + 40,), 7.0, dtype=dtype, device="cuda")
+        out = buf[first:first + want.numel()].view(want.shape)
+        assert afa.afa_paged(*b.args(), out=out) is out
+        assert torch.equal(out, want), first
+        assert (buf[:first] == 7.0).all() and (buf[first + want.numel():] == 7.0).all()
