@@ -379,7 +379,8 @@ extern "C" int afa_ago_rotate_axes(const void* q, const long long* q_strides, vo
     S.turn = 1;
     a.groups += S.groups;
     wide = wide && aligned(S.src, 16, dtype_size(dtype), {st[0], st[1], st[2]}) && aligned(S.dst, 16, 1, {});
-    if (!aligned(S.src, 2 * dtype_size(dtype), dtype_size(dtype), {st[0], st[1], st[2]}))
+    if (!aligned(S.src, 2 * dtype_size(dtype), dtype_size(dtype), {st[0], st[1], st[2]}) ||
+        !aligned(S.dst, 2 * dtype_size(dtype), 1, {}))
       return invalid("afa_ago_rotate_axes: rows must start at a channel pair's alignment");
   }
   a.c = c;

@@ -226,8 +226,9 @@ AFA_API int afa_ago_rotate(const void* q, const void* k, void* q_out, void* k_ou
  *                 int32, or int64 when positions_64, strides (axis, batch,
  *                 token); a position the tables (table_len, dim / 2) do not
  *                 hold makes its pairs NaN. backward: turns the other way, the
- *                 gradient. At most four axes. Arithmetic in float32 (float64
- *                 for AFA_F64), one rounding.
+ *                 gradient. At most four axes. Rows in and out start on a
+ *                 channel pair (twice the element's size). Arithmetic in
+ *                 float32 (float64 for AFA_F64), one rounding.
  */
 AFA_API int afa_ago_rotate_axes(const void* q, const long long* q_strides, void* q_out, int q_heads, const void* k,
                                 const long long* k_strides, void* k_out, int k_heads, const void* c, const void* s,

@@ -258,3 +258,14 @@ def test_oracle_causal_attention_is_the_dense_one():
     out, _ = po.attend(q, *caches, table, [21], [0, 21])
     dense = orc.afa(*(x.transpose(1, 0, 2)[None] for x in (q, k.repeat(2, 1), v.repeat(2, 1))), causal=True)
     assert np.max(np.abs(out.transpose(1, 0, 2)[None] - dense)) < 1e-13
+
+
+def test_c_rotation_refuses_outputs_off_a_channel_pair():
+    """The kernel stores a pair at a time: an output off one would be a misaligned access."""
+    lib = _lib.load()
+    three, secs = (ctypes.c_longlong * 3)(2, 2, 2), (ctypes.c_int * 1)(1)
+    for dtype, size in ((_lib.AFA_BF16, 2), (_lib.AFA_F32, 4), (_lib.AFA_F64, 8)):
+        for q_out, k_out in ((4096 + size, 4096), (4096, 4096 + size)):
+            assert lib.afa_ago_rotate_axes(4096, three, q_out, 1, 4096, three, k_out, 1, 4096, 4096, _lib.AFA_F32, 4,
+                                           4096, three, 0, secs, 1, 1, 1, 2, 2, 0, dtype, None) == _lib.AFA_ERR_INVALID
+            assert b"alignment" in lib.afa_last_error()
