@@ -98,6 +98,23 @@ __device__ __forceinline__ void tmem_ld_few(uint32_t taddr, uint32_t (&r)[N]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(taddr));
 }
 
+// Clears the rows of a query tile behind the unit's: TMA has put the next
+// tokens' queries there, or nothing (unit_rows may be less than NT). Their
+// outputs go nowhere, but their scores would have a say in which form a chunk of
+// weights is computed in (see kTrTail), so that a row's last bits depended on
+// other requests and on what the shared memory held before. The warp that issues
+// the products calls it after the tile has arrived.
+template <int KSUB, int NT>
+__device__ __forceinline__ void clear_q_rows(uint8_t* tile, int rows, int lane) {
+  if (rows >= NT) return;
+  for (int x = rows * 8 + lane; x < NT * 8; x += 32)
+#pragma unroll
+    for (int h = 0; h < KSUB; ++h)
+      st_shared_v4(smem_u32(tile + h * NT * 128 + x * 16), make_uint4(0u, 0u, 0u, 0u));
+  fence_proxy_async_shared();
+  __syncwarp();
+}
+
 // Sums of 8 values over the warp's lanes: lane l returns value l / 4's.
 __device__ __forceinline__ float reduce8(const float* v, int lane) {
   float x[8];
@@ -134,7 +151,10 @@ __device__ __forceinline__ void map8(const uint32_t* sv, float scale, unsigned s
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     s[e] = __fmul2_rn(make_float2(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), sc);
-    least = fminf(least, fminf(s[e].x, s[e].y));
+    // Of the scores that count: keys behind the request's last token may be anything.
+    const float x = !MASK || (seen & (1u << (2 * e))) ? s[e].x : 0.f;
+    const float y = !MASK || (seen & (2u << (2 * e))) ? s[e].y : 0.f;
+    least = fminf(least, fminf(x, y));
   }
   if (__any_sync(0xffffffffu, least < kTrTail)) {
 #pragma unroll
@@ -308,6 +328,8 @@ __global__ void __launch_bounds__(608, 1)
         if (!(ok = __all_sync(0xffffffffu, mbar_wait(q_full + (s_qn & 1), (s_qn >> 1) & 1, a.status,
                                                      kDevTimeoutMma))))
           return false;
+        clear_q_rows<C::KSUB, NT>(smem + C::Q_OFF + (s_qn & 1) * C::Q_BYTES,
+                                  uniform(min(sp.r.n * a.G - sp.u * a.unit_rows, a.unit_rows)), lane);
       }
       return ok = __all_sync(0xffffffffu, mbar_wait(kv_full + kpos.slot, kpos.phase, a.status, kDevTimeoutMma));
     };

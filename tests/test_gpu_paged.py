@@ -696,3 +696,43 @@ def test_attention_out_that_starts_anywhere(name, dtype, dim):
         assert afa.afa_paged(*b.args(), out=out) is out
         assert torch.equal(out, want), first
         assert (buf[:first] == 7.0).all() and (buf[first + want.numel():] == 7.0).all()
+
+
+def surroundings(seed, dim, group, new, dtype=BF):
+    """Short requests of weak scores (none below -4, so that anything that reaches them shows), every other one idle,
+    with room behind their rows of q and behind their last tokens in the cache."""
+    rng = np.random.default_rng(seed)
+    lens = [130, 0, 1, 0, 77, 0, 260, 0]
+    n = [min(new, x) for x in lens]
+    b = Batch(seed, n, lens, 2, group, dim, 32, dtype)
+    q, k, v, table, slens, cu, _ = b.args()
+    behind = [torch.isnan(x[..., :1]) for x in (k, v)]
+    q = torch.cat((q * 0.5, torch.zeros((4, *q.shape[1:]), dtype=dtype, device="cuda")))
+    noise = dev(rng.standard_normal(k.shape), dtype) * 20
+
+    def call(beside, sign):
+        """Rows of q of no request and cache rows of no token, as `beside` times something."""
+        qq = q.clone()
+        qq[int(cu[-1]):] = sign * beside * dev(rng.standard_normal((4, *q.shape[1:])), dtype)
+        kk, vv = (torch.where(m, beside * noise, x) for m, x in zip(behind, (k, v)))
+        return afa.afa_paged(qq, kk, vv, table, slens, cu, return_denominator=True), int(cu[-1])
+
+    return call
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("group,new", [(1, 1), (3, 1), (4, 1), (5, 1), (6, 1), (7, 1), (7, 4), (3, 7), (5, 6), (16, 1),
+                                       (4, 40), (7, 40)])
+def test_attention_does_not_depend_on_its_surroundings(dim, group, new):
+    """The same bits whatever lies in rows of q of no request, behind a request's last token, and in the shared memory
+    that the launch before left (groups that do not divide 16 or 32 leave rows of the query tile unwritten)."""
+    call = surroundings(20 + group, dim, group, new)
+    other = surroundings(50, dim, 16, 2)
+    results = []
+    for beside in (0.0, 1.0, 30.0, float("nan")):
+        other(beside, 1)
+        (out, den), t = call(beside, 1)
+        results.append((out[:t].clone(), den[:t].clone()))
+    assert _lib.device_status(out.device) == 0
+    for out, den in results[1:]:
+        assert torch.equal(den, results[0][1]) and torch.equal(out, results[0][0])
