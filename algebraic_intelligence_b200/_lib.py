@@ -52,7 +52,7 @@ SIGNATURES = {
     "afa_paged_commit": (_c_int, [_c_void_p] * 5 + [_c_ll] + [_c_void_p] * 3 + [_c_ll, _c_void_p] + [_c_int] * 9 +
                          [_c_void_p]),
     "afa_paged": (_c_int, [_c_void_p] * 9 + [_c_ll] + [_c_void_p] * 3 + [_c_ll] + [_c_int] * 10 +
-                  [_c_float, _c_void_p, _c_size, _c_void_p]),
+                  [_c_double, _c_void_p, _c_size, _c_void_p]),
     "afa_paged_workspace_bytes": (_c_size, [_c_int] * 5),
     "algebraic_softmax_fwd": (_c_int, [_c_void_p, _c_void_p, _c_ll, _c_int, _c_int, _c_double, _c_double,
                                        _c_void_p]),

@@ -504,7 +504,7 @@ extern "C" int afa_paged(const void* q, const long long* q_strides, const void* 
                          const int* block_table, long long table_stride, const int* seq_lens, const int* cu_tokens,
                          const void* ancestors, long long ancestors_stride, int ancestor_words, int batch, int tokens,
                          int q_heads, int kv_heads, int D, int table_cols, int page_size, int num_pages, int dtype,
-                         float sink_omega, void* workspace, size_t workspace_bytes, void* stream) {
+                         double sink_omega, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace afa;
   if (dtype == AFA_F16)
     return set_last_error(AFA_ERR_DTYPE, "float16 is not supported: rho(s)^8 overflows float16 for s > 2.4; use "
@@ -517,7 +517,10 @@ extern "C" int afa_paged(const void* q, const long long* q_strides, const void* 
   if (q_heads % kv_heads != 0) return invalid("query heads must be a multiple of the cache's heads");
   if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)) != 0)
     return invalid("page_size must be a power of two from 16 to 256");
-  if (!(std::isfinite(sink_omega) && sink_omega >= 0.f)) return invalid("sink_omega must be finite and nonnegative");
+  // In the type that the sums have: float64 keeps all of it.
+  const float sink = static_cast<float>(sink_omega);
+  if (!(sink_omega >= 0.0 && (dtype == AFA_F64 ? std::isfinite(sink_omega) : std::isfinite(sink))))
+    return invalid("sink_omega must be finite and nonnegative");
   if (static_cast<long long>(table_cols) * page_size > INT_MAX - 65536)
     return invalid("afa_paged: a block table row may hold at most 2^31 - 65537 tokens");
   if (static_cast<long long>(tokens) * q_heads > INT_MAX / 2) return invalid("afa_paged: too many query rows");
@@ -570,8 +573,8 @@ extern "C" int afa_paged(const void* q, const long long* q_strides, const void* 
   a.num_pages = num_pages;
   a.scale_d = 1.0 / std::sqrt(static_cast<double>(D));
   a.scale = static_cast<float>(a.scale_d);
-  a.sink_d = static_cast<double>(sink_omega);
-  a.sink = sink_omega;
+  a.sink_d = sink_omega;
+  a.sink = sink;
   a.meta = static_cast<int*>(workspace);
   a.frag = static_cast<char*>(workspace) + kMetaBytes;
   a.status = device_status_ptr();

@@ -362,7 +362,7 @@ AFA_API int afa_paged(const void* q, const long long* q_strides, const void* k_c
                       const int* block_table, long long table_stride, const int* seq_lens, const int* cu_tokens,
                       const void* ancestors, long long ancestors_stride, int ancestor_words, int batch, int tokens,
                       int q_heads, int kv_heads, int D, int table_cols, int page_size, int num_pages, int dtype,
-                      float sink_omega, void* workspace, size_t workspace_bytes, void* stream);
+                      double sink_omega, void* workspace, size_t workspace_bytes, void* stream);
 AFA_API size_t afa_paged_workspace_bytes(int tokens, int q_heads, int kv_heads, int D, int dtype);
 AFA_API int afa_paged_commit(void* k_cache, const long long* k_strides, void* v_cache, const long long* v_strides,
                              const int* block_table, long long table_stride, const int* base_lens,

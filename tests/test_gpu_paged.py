@@ -736,3 +736,19 @@ def test_attention_does_not_depend_on_its_surroundings(dim, group, new):
     assert _lib.device_status(out.device) == 0
     for out, den in results[1:]:
         assert torch.equal(den, results[0][1]) and torch.equal(out, results[0][0])
+
+
+@pytest.mark.parametrize("sink", [0.3, 1e-300, 2.0 ** 200])
+def test_attention_float64_keeps_its_sink(sink):
+    """float64 throughout: a sink that float32 does not hold is not rounded to it."""
+    b = Batch(14, [1, 9, 3], [1, 200, 0], 2, 3, 64, 16, F64)
+    out, den = b.check(sink)
+    assert torch.equal(den[-3:], torch.full_like(den[-3:], sink))
+    want, wden = po.attend(host(b.q), *(np.nan_to_num(host(x)) for x in b.caches), b.table, b.lens, b.cu, None, sink)
+    assert np.max(np.abs(host(den) / wden - 1)) <= TOL[F64]
+
+
+def test_attention_float32_refuses_a_sink_it_cannot_hold():
+    b = Batch(15, [1], [20], 1, 1, 64, 16, F32)
+    with pytest.raises(ValueError, match="sink_omega"):
+        b.check(2.0 ** 200)
