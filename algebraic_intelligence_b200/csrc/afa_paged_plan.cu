@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const __grid_c
     cu[a.B] = T;
     if (blockIdx.x == 0) {
       a.cu[a.B] = T;
-      a.free_out[0] = fc + F - A;
+      a.free_out[0] = min(fc + F - A, a.N);  // what finds no room on the stack is not on it
     }
   }
   __syncthreads();

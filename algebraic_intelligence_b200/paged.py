@@ -117,7 +117,9 @@ def paged_plan(block_table, page_counts, seq_lens, new_lens, free_pages, free_co
     request holds behind ``need`` (it ended, or drafted tokens were rejected)
     are released onto the stack in request order; then the requests that need
     more take them from its top, in request order (a page belongs to one
-    request: one that two held would join the stack twice). ``block_table`` and
+    request: one that two held would join the stack twice). ``free_pages`` has
+    room for every page of the cache, since all may be free at once: a released
+    page that finds no room is lost, and not counted. ``block_table`` and
     ``free_pages`` are updated in place; lengths and counts come back in new
     tensors, so a call with the same inputs gives the same step.
 

@@ -290,7 +290,9 @@ AFA_API int afa_decode_noalloc(const void* q, const void* k_cache, const void* v
  *                 need = ceil((seq_lens + new_lens) / page_size), pages behind
  *                 `need` are released: in request order they join the top of
  *                 the stack free_pages[0 .. free_count). Then the requests that
- *                 need more take them from the top, in request order. A request
+ *                 need more take them from the top, in request order. free_pages
+ *                 has room for every page that can be free at once: released
+ *                 pages behind its end are lost, and not counted. A request
  *                 is refused, keeping what it holds, when its row of the table
  *                 (table_cols) or, with parents, a tree of `nodes` is too
  *                 small for it, when the tokens asked for up to and with it

@@ -32,6 +32,7 @@ def plan(table, held, lens, new, stack, free, page, max_tokens, parents=None):
             continue
         for j in range(grow):
             table[b, held[b] + j] = state.pop()
+    state = state[:len(stack)]  # released pages that find no room are lost
     if len(state) > free:
         stack[int(free):len(state)] = state[int(free):]
     slots, rows, positions, words = [], [], [], []

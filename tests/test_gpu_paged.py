@@ -752,3 +752,18 @@ def test_attention_float32_refuses_a_sink_it_cannot_hold():
     b = Batch(15, [1], [20], 1, 1, 64, 16, F32)
     with pytest.raises(ValueError, match="sink_omega"):
         b.check(2.0 ** 200)
+
+
+def test_plan_stack_without_room():
+    """Released pages that find no room are not counted, and nothing is written behind the stack."""
+    full = np.arange(8, dtype=np.int32).reshape(2, 4)
+    for size, free in ((3, 0), (5, 5), (4, 3), (7, 0)):
+        r = check_plan(full, [4, 3], [0, 0], [0, 0], np.arange(20, 20 + size, dtype=np.int32), free, 16, 0)
+        assert r["free_count"][0] == size
+    # pages that go on to another request in the same step need none
+    r = check_plan(full, [4, 1], [1, 16], [0, 40], np.full(1, 30, np.int32), 1, 16, 64)
+    assert r["granted"].all() and r["free_count"][0] == 1 and r["page_counts"][1] == 4
+    buf = i32(np.full(6, 77))
+    tables = i32(full), i32([4, 3]), i32([0, 0]), i32([0, 0])
+    p = afa.paged_plan(*tables, buf[:3], i32([1]), 16, 0)
+    assert int(p.free_count) == 3 and (buf[3:] == 77).all()
