@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import numpy as np
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 
 class Staged:
@@ -55,3 +56,10 @@ def host_checks_float(*arrays) -> None:
             ok = dt.is_floating_point
         if not ok:
             raise TypeError("expected a floating point array")
+
+
+def refuse_tangents(what, *arrays) -> None:
+    """ValueError for inputs with a forward-mode tangent, which a kernel would drop without a sign."""
+    for a in arrays:
+        if isinstance(a, torch.Tensor) and unpack_dual(a).tangent is not None:
+            raise ValueError(f"{what} has no forward-mode derivative")

@@ -29,7 +29,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._tensors import Staged, host_checks_float
+from ._tensors import Staged, host_checks_float, refuse_tangents
 
 __all__ = ["CayleyRotary", "build_cayley_rotary_matrix", "apply_ago_rotations", "apply_ago_rotations_axes"]
 
@@ -206,6 +206,7 @@ def axis_arguments(rotary_params, positions, sections, dim, shape, device) -> Ax
                          f"{tuple(s.shape)}")
     if c.requires_grad or s.requires_grad:
         raise ValueError("the rotary tables have no gradient")
+    refuse_tangents("a rotary table", c, s)
     p = positions if isinstance(positions, torch.Tensor) else torch.as_tensor(np.asarray(positions))
     if p.dtype != torch.int32 and p.dtype != torch.int64:
         raise TypeError("positions must be int32 or int64")
@@ -298,7 +299,7 @@ def apply_ago_rotations_axes(q, k, rotary_params, positions, sections):
     NaN on the device. ``rotary_params`` as in ``apply_ago_rotations``, (positions,
     dim / 2). Unlike there the tables keep their dtype: the arithmetic is
     float32 (float64 for float64 inputs) with one rounding, which a bfloat16
-    table would limit to 2^-9. Differentiable in q and k (before a backward pass
+    table would limit to 2^-9. Differentiable in q and k by backward passes (before one
     is captured into a CUDA graph, release what was computed from the same
     leaves outside of it: PyTorch would wait for those leaves' stream). Returns
     contiguous (q_rot, k_rot).
@@ -315,6 +316,7 @@ def apply_ago_rotations_axes(q, k, rotary_params, positions, sections):
     if q.shape[head] == 0 or (k is not None and k.shape[head] == 0):
         raise ValueError("q and k need at least one head")
     host_checks_float(*(t for t in (q, k) if t is not None))
+    refuse_tangents("apply_ago_rotations_axes", q, k)
     if k is not None and k.dtype != q.dtype:
         raise TypeError("q and k must share a dtype")
     on_gpu = all(t is None or (isinstance(t, torch.Tensor) and t.is_cuda) for t in (q, k))

@@ -29,6 +29,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
+from ._tensors import refuse_tangents
 from .ago import axis_arguments
 
 __all__ = ["PagedPlan", "paged_plan", "paged_append", "afa_paged", "paged_commit", "paged_workspace_bytes"]
@@ -78,6 +79,7 @@ def _no_gradient(what, *tensors):
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise ValueError(f"{what} has no gradient: call it under torch.no_grad()")
+    refuse_tangents(what, *tensors)
 
 
 def _caches(k_cache, v_cache, ndims=(4,)):

@@ -269,3 +269,25 @@ def test_c_rotation_refuses_outputs_off_a_channel_pair():
             assert lib.afa_ago_rotate_axes(4096, three, q_out, 1, 4096, three, k_out, 1, 4096, 4096, _lib.AFA_F32, 4,
                                            4096, three, 0, secs, 1, 1, 1, 2, 2, 0, dtype, None) == _lib.AFA_ERR_INVALID
             assert b"alignment" in lib.afa_last_error()
+
+
+def test_forward_mode_tangents_are_refused():
+    """Not dropped: also of tensors that want no gradient, and where no gradients are recorded."""
+    from torch.autograd import forward_ad as fw
+    f = torch.float32
+
+    def dual(*shape):
+        return fw.make_dual(_z(*shape, dtype=f), torch.ones(shape))
+
+    x = torch.zeros(2, 3, 5, 8)
+    tables = torch.ones(9, 4), torch.zeros(9, 4)
+    cache, q = _z(5, 2, 16, 64, dtype=f), _z(3, 4, 64, dtype=f)
+    with fw.dual_level(), torch.no_grad():
+        for call in (lambda: _rotate(q=dual(2, 3, 5, 8), k=x[:, :1]), lambda: _rotate(q=x, k=dual(2, 1, 5, 8)),
+                     lambda: _rotate(q=x, k=None, rotary_params=(dual(9, 4), tables[1])),
+                     lambda: _append(k=dual(3, 2, 8)), lambda: _append(v_cache=dual(5, 2, 16, 8)),
+                     lambda: _commit(k_cache=dual(5, 2, 16, 8)),
+                     lambda: _attend(q=dual(3, 4, 64), k_cache=cache, v_cache=cache),
+                     lambda: _attend(q=q, k_cache=cache, v_cache=dual(5, 2, 16, 64))):
+            with pytest.raises(ValueError, match="no forward-mode derivative"):
+                call()
