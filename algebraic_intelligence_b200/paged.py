@@ -24,6 +24,7 @@ attributes and resolves the device status word.
 """
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -101,6 +102,30 @@ def _caches(k_cache, v_cache, ndims=(4,)):
     if k_cache.stride()[-1] != 1 or v_cache.stride()[-1] != 1:
         raise ValueError("a cache row's channels must be contiguous")
     return pages, heads, page_size, dim
+
+
+@functools.lru_cache(maxsize=4096)
+def _apart(shape, strides, behind) -> bool:
+    """Whether the elements of a strided view, and of a second one ``behind`` elements further, all lie apart. (Views
+    made by slicing, indexing and transposing do: each stride passes what the smaller ones span.)"""
+    span = 0
+    for stride, n in sorted((*zip(strides, shape), (behind, 2))):
+        if n > 1:
+            if stride <= span:
+                return False
+            span += stride * (n - 1)
+    return True
+
+
+def _written(k_cache, v_cache):
+    """Refuses caches whose rows share memory, as an expanded one's: moves and writes of rows would race."""
+    behind = abs(k_cache.data_ptr() - v_cache.data_ptr()) // k_cache.element_size()
+    if k_cache.stride() == v_cache.stride():
+        apart = _apart(k_cache.shape, k_cache.stride(), behind)
+    else:
+        apart = behind > 0 and all(_apart(t.shape, t.stride(), 1 << 62) for t in (k_cache, v_cache))
+    if not apart:
+        raise ValueError("the caches are written to: their rows must not share memory")
 
 
 def _rows(t):
@@ -193,7 +218,7 @@ def paged_append(k, v, k_cache, v_cache, slots, q=None, rotary_params=None, posi
     ``apply_ago_rotations_axes`` the keys are rotated, and so is ``q`` (tokens,
     heads, dim), which comes back; without q the result is None. The caches may
     be strided views (such as a (pages, page_size, heads, dim) cache
-    transposed).
+    transposed) whose rows lie apart.
     """
     pages, heads, page_size, dim = _caches(k_cache, v_cache)
     if k.ndim != 3 or k.shape != v.shape or k.shape[1:] != (heads, dim):
@@ -217,6 +242,7 @@ def paged_append(k, v, k_cache, v_cache, slots, q=None, rotary_params=None, posi
         raise ValueError("q, positions and sections go with rotary_params")
     _no_gradient("paged_append", k, v, q, k_cache, v_cache)
     dev = _one_device(k_cache, v_cache, k, v, q, slots)
+    _written(k_cache, v_cache)
     axes = axis_arguments(rotary_params, positions, sections, dim, (tokens,), dev) if rotary_params is not None \
         else None
     k, v = _rows(k), _rows(v)
@@ -361,6 +387,7 @@ def paged_commit(k_cache, v_cache, block_table, base_lens, seq_lens, accepted) -
         raise ValueError("an accepted path may have at most 256 tokens")
     _no_gradient("paged_commit", k_cache, v_cache)
     dev = _one_device(k_cache, v_cache, block_table, base_lens, seq_lens, accepted)
+    _written(k_cache, v_cache)
     block_table, accepted = _rows(block_table), _rows(accepted)
     base_lens, seq_lens = base_lens.contiguous(), seq_lens.contiguous()
     lens = torch.empty(b, dtype=torch.int32, device=dev)

@@ -291,3 +291,41 @@ def test_forward_mode_tangents_are_refused():
                      lambda: _attend(q=q, k_cache=cache, v_cache=dual(5, 2, 16, 64))):
             with pytest.raises(ValueError, match="no forward-mode derivative"):
                 call()
+
+
+@pytest.mark.parametrize("layers", [0, 2])
+def test_caches_whose_rows_share_memory_are_refused(layers, monkeypatch):
+    """They are written to. Ordinary views, also both caches in one buffer, are not (here they get as far as the
+    launch, with tensors that only claim to be on a GPU)."""
+    from algebraic_intelligence_b200 import paged
+    monkeypatch.setattr(paged, "_one_device", lambda *tensors: torch.device("cpu"))
+
+    class Launched(Exception):
+        pass
+
+    def launch(*args):
+        raise Launched
+
+    monkeypatch.setattr(_lib, "call", launch)
+    f, lead = torch.float32, (layers,) if layers else ()
+    z = lambda *shape: _z(*lead, *shape, dtype=f)  # noqa: E731
+    calls = [_commit] if layers else [_commit, _append]
+    plain = z(5, 2, 16, 8)
+    wide = z(5, 2, 2, 16, 8)
+    fused, pool = z(5, 16, 2, 24), z(10, 2, 16, 8)
+    for k, v in ((plain, z(5, 2, 16, 8)), (z(5, 16, 2, 8).transpose(-3, -2), z(5, 16, 2, 8).transpose(-3, -2)),
+                 (z(5, 16, 2, 8).transpose(-3, -2), plain), (wide.select(-4, 0), wide.select(-4, 1)),
+                 (wide.select(-4, 1), wide.select(-4, 0)), (wide.select(-3, 0), wide.select(-3, 1)),
+                 (fused[..., :8].transpose(-3, -2), fused[..., 16:].transpose(-3, -2)),
+                 (pool[..., ::2, :, :, :], pool[..., 1::2, :, :, :]), (pool[..., 5:, :, :, :], pool[..., :5, :, :, :])):
+        for call in calls:
+            with pytest.raises(Launched):
+                call(k_cache=k, v_cache=v)
+    spread = z(5, 1, 16, 8).expand(*lead, 5, 2, 16, 8)
+    pages = z(1, 2, 16, 8).expand(*lead, 5, 2, 16, 8)
+    window = torch.zeros(4000).as_strided((*lead, 5, 2, 16, 8), (*(2000,) * len(lead), 256, 128, 4, 1))
+    for k, v in ((spread, plain), (plain, pages), (plain, plain), (plain, window), (window, window),
+                 (wide.select(-4, 0), wide.select(-4, 0)), (spread, spread)):
+        for call in calls:
+            with pytest.raises(ValueError, match="share memory"):
+                call(k_cache=k, v_cache=v)
