@@ -161,8 +161,10 @@ __global__ void __launch_bounds__(kRowThreads, 4) paged_rows_kernel(const __grid
           for (int p = 0; p < P; ++p) {
             if (p0 + p >= end) continue;
             const A x0 = static_cast<A>(to_acc(y[2 * p])), x1 = static_cast<A>(to_acc(y[2 * p + 1]));
-            y[2 * p] = from_acc<T>(cc[p] * x0 - ss[p] * x1);
-            y[2 * p + 1] = from_acc<T>(ss[p] * x0 + cc[p] * x1);
+            // Which product is rounded is said here, not left to the compiler: the wide
+            // and the narrow kernel give the same bits.
+            y[2 * p] = from_acc<T>(fma(cc[p], x0, -(ss[p] * x1)));
+            y[2 * p + 1] = from_acc<T>(fma(ss[p], x0, cc[p] * x1));
           }
           memcpy(&in[j], y, sizeof(V));
         }

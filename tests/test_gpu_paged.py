@@ -767,3 +767,28 @@ def test_plan_stack_without_room():
     tables = i32(full), i32([4, 3]), i32([0, 0]), i32([0, 0])
     p = afa.paged_plan(*tables, buf[:3], i32([1]), 16, 0)
     assert int(p.free_count) == 3 and (buf[3:] == 77).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32, F64])
+def test_rotation_bits_do_not_depend_on_alignment(dtype):
+    """Rows on 16 bytes and rows on a channel pair, forward, gradient and into the cache."""
+    rng = np.random.default_rng(17)
+    c, s = tables(64, 40, F32)
+    x = dev(rng.standard_normal((2, 3, 50, 66)), dtype)
+    pos = dev(rng.integers(0, 40, (2, 2, 50)))
+
+    def turned(q):
+        q = q.detach().requires_grad_(True)
+        y, _ = afa.apply_ago_rotations_axes(q, None, (c, s), pos, (20, 11))
+        return y.detach(), torch.autograd.grad(y, q, q.detach())[0]
+
+    for a, b in zip(turned(x[..., 2:]), turned(x[..., 2:].contiguous())):
+        assert torch.equal(a, b)
+    rows = x.transpose(1, 2).reshape(100, 3, 66)[..., 2:]
+    caches = [torch.zeros((8, 3, 16, 64), dtype=dtype, device="cuda") for _ in range(4)]
+    slots = dev(rng.permutation(128)[:100])
+    args = dict(rotary_params=(c, s), positions=pos.reshape(2, 100), sections=(20, 11))
+    got = afa.paged_append(rows, rows, *caches[:2], slots, q=rows, **args)
+    rows = rows.contiguous()
+    assert torch.equal(got, afa.paged_append(rows, rows, *caches[2:], slots, q=rows, **args))
+    assert torch.equal(caches[0], caches[2]) and torch.equal(caches[1], caches[3])
