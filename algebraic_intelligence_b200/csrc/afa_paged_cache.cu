@@ -237,6 +237,10 @@ bool aligned(const void* p, size_t unit, size_t esize, std::initializer_list<lon
   return true;
 }
 
+// The stride of an axis of one entry says nothing and is never multiplied by
+// anything but 0: it does not count against the alignment of rows.
+long long used(long long stride, int entries) { return entries > 1 ? stride : 0; }
+
 // The axes' channel pairs as running ends; false when they do not fit.
 bool set_axes(RowArgs& a, const int* sections, int axes) {
   int at = 0;
@@ -370,9 +374,9 @@ extern "C" int afa_ago_rotate_axes(const void* q, const long long* q_strides, vo
     RowSet& S = a.set[i];
     S.src = i ? k : q;
     S.dst = i ? k_out : q_out;
-    S.s_b = st[0];
-    S.s_t = st[1];
-    S.s_h = st[2];
+    S.s_b = used(st[0], batch);
+    S.s_t = used(st[1], tokens);
+    S.s_h = used(st[2], heads);
     S.d_b = static_cast<long long>(heads) * tokens * dim;
     S.d_t = token_major ? static_cast<long long>(heads) * dim : dim;
     S.d_h = token_major ? dim : static_cast<long long>(tokens) * dim;
@@ -380,8 +384,8 @@ extern "C" int afa_ago_rotate_axes(const void* q, const long long* q_strides, vo
     S.groups = (heads + kHeadsPerThread - 1) / kHeadsPerThread;
     S.turn = 1;
     a.groups += S.groups;
-    wide = wide && aligned(S.src, 16, dtype_size(dtype), {st[0], st[1], st[2]}) && aligned(S.dst, 16, 1, {});
-    if (!aligned(S.src, 2 * dtype_size(dtype), dtype_size(dtype), {st[0], st[1], st[2]}) ||
+    wide = wide && aligned(S.src, 16, dtype_size(dtype), {S.s_b, S.s_t, S.s_h}) && aligned(S.dst, 16, 1, {});
+    if (!aligned(S.src, 2 * dtype_size(dtype), dtype_size(dtype), {S.s_b, S.s_t, S.s_h}) ||
         !aligned(S.dst, 2 * dtype_size(dtype), 1, {}))
       return invalid("afa_ago_rotate_axes: rows must start at a channel pair's alignment");
   }
@@ -439,12 +443,12 @@ extern "C" int afa_paged_append(const void* k, const long long* k_strides, const
     S.src = i == 0 ? k : i == 1 ? v : q;
     S.dst = i == 0 ? k_cache : i == 1 ? v_cache : q_out;
     S.s_b = 0;
-    S.s_t = st[0];
-    S.s_h = st[1];
     S.heads = i == 2 ? q_heads : kv_heads;
-    S.d_b = i == 2 ? 0 : cs[0];
+    S.s_t = used(st[0], tokens);
+    S.s_h = used(st[1], S.heads);
+    S.d_b = i == 2 ? 0 : used(cs[0], num_pages);
     S.d_t = i == 2 ? static_cast<long long>(q_heads) * dim : cs[2];
-    S.d_h = i == 2 ? dim : cs[1];
+    S.d_h = i == 2 ? dim : used(cs[1], kv_heads);
     S.groups = (S.heads + kHeadsPerThread - 1) / kHeadsPerThread;
     S.turn = i != 1 && c;
     S.cache = i != 2;
@@ -501,13 +505,13 @@ extern "C" int afa_paged_commit(void* k_cache, const long long* k_strides, void*
   a.lens = seq_lens;
   a.accepted = accepted;
   a.lens_out = lens_out;
-  a.k_l = k_strides[0];
-  a.k_p = k_strides[1];
-  a.k_h = k_strides[2];
+  a.k_l = used(k_strides[0], layers);
+  a.k_p = used(k_strides[1], num_pages);
+  a.k_h = used(k_strides[2], kv_heads);
   a.k_r = k_strides[3];
-  a.v_l = v_strides[0];
-  a.v_p = v_strides[1];
-  a.v_h = v_strides[2];
+  a.v_l = used(v_strides[0], layers);
+  a.v_p = used(v_strides[1], num_pages);
+  a.v_h = used(v_strides[2], kv_heads);
   a.v_r = v_strides[3];
   a.table_ld = table_stride;
   a.acc_ld = accepted_stride;

@@ -792,3 +792,34 @@ def test_rotation_bits_do_not_depend_on_alignment(dtype):
     rows = rows.contiguous()
     assert torch.equal(got, afa.paged_append(rows, rows, *caches[2:], slots, q=rows, **args))
     assert torch.equal(caches[0], caches[2]) and torch.equal(caches[1], caches[3])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_strides_of_single_entries_do_not_matter(dtype):
+    """One token, one head, one batch row, one page: the stride of such an axis is never used, whatever it is."""
+    rng = np.random.default_rng(16)
+    c, s = tables(32, 16, F32)
+    rows = dev(rng.standard_normal((3, 6 * 32 + 1)), dtype)[:, :192].unflatten(1, (6, 32))  # a projection of odd width
+    q, k, v = rows[2:].split((4, 1, 1), 1)
+    assert q.stride(0) % 2 == 1 and k.stride(0) % 2 == 1
+    pos = dev([[3]])
+    got = afa.apply_ago_rotations_axes(q, k, (c, s), pos, (16,))
+    want = afa.apply_ago_rotations_axes(q.clone(), k.clone(), (c, s), pos, (16,))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    x = dev(rng.standard_normal((1, 1, 5, 32)), dtype)
+    odd = x.as_strided(x.shape, (331, 77, 32, 1))
+    assert torch.equal(afa.apply_ago_rotations_axes(odd, None, (c, s), dev(np.arange(5)[None]), (16,))[0],
+                       afa.apply_ago_rotations_axes(x, None, (c, s), dev(np.arange(5)[None]), (16,))[0])
+    caches = [torch.zeros((1, 1, 16, 32), dtype=dtype, device="cuda") for _ in range(4)]
+    views = [t.as_strided(t.shape, (1037, 519, 32, 1)) for t in caches[:2]]
+    args = dict(q=q, rotary_params=(c, s), positions=pos, sections=(16,))
+    assert torch.equal(afa.paged_append(k, v, *views, dev([7]), **args), want[0])
+    afa.paged_append(k.clone(), v.clone(), *caches[2:], dev([7]))
+    assert torch.equal(caches[0][0, 0, 7], want[1][0, 0]) and torch.equal(caches[1], caches[3])
+    got = afa.afa_paged(q, *views, i32([[0]]), i32([8]), i32([0, 1]))
+    assert torch.equal(got, afa.afa_paged(q.clone(), *caches[:2], i32([[0]]), i32([8]), i32([0, 1])))
+    caches[0][0, 0, :8], caches[1][0, 0, :8] = (dev(rng.standard_normal((8, 32)), dtype) for _ in range(2))
+    before = [t.clone() for t in caches[:2]]
+    assert int(afa.paged_commit(*views, i32([[0]]), i32([2]), i32([8]), i32([[1, 3, -1]]))) == 4
+    for t, b in zip(caches, before):
+        assert torch.equal(t[0, 0, 2:4], b[0, 0, [3, 5]]) and torch.equal(t[0, 0, 4:], b[0, 0, 4:])
