@@ -28,6 +28,7 @@ import functools
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._tensors import refuse_tangents
@@ -204,6 +205,7 @@ def paged_plan(block_table, page_counts, seq_lens, new_lens, free_pages, free_co
         per_request + 8 * b + 4, behind - 4, behind + 4 * w, behind, b, cols, page_size, free_pages.shape[0], t, nodes)
     if rc:
         _lib.check(rc, "afa_paged_plan")
+    increment_version((block_table, free_pages))
     return PagedPlan(slots.view(torch.int64), rows, positions, cu, lens_out, held_out, free_out,
                      granted.view(torch.bool)[:b], ancestors.view(max_tokens, words) if nodes else None)
 
@@ -269,6 +271,7 @@ def paged_append(k, v, k_cache, v_cache, slots, q=None, rotary_params=None, posi
         _lib.dtype_code(k_cache.dtype))
     if rc:
         _lib.check(rc, "afa_paged_append")
+    increment_version((k_cache, v_cache))
     return out
 
 
@@ -335,7 +338,8 @@ def afa_paged(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, ancestors=N
     dev = _one_device(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, ancestors, out, workspace)
     q, block_table = _rows(q), _rows(block_table)
     seq_lens, cu_tokens = seq_lens.contiguous(), cu_tokens.contiguous()
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=dev)
     den = torch.empty((tokens, heads), dtype=_lib.accum_dtype(q.dtype), device=dev) if return_denominator else None
     lib = _lib.load()
@@ -355,6 +359,8 @@ def afa_paged(q, k_cache, v_cache, block_table, seq_lens, cu_tokens, ancestors=N
         float(sink_omega), workspace.data_ptr(), need)
     if rc:
         _lib.check(rc, "afa_paged")
+    if given:
+        increment_version(out)
     return (out, den) if return_denominator else out
 
 
@@ -401,4 +407,5 @@ def paged_commit(k_cache, v_cache, block_table, base_lens, seq_lens, accepted) -
         _lib.dtype_code(k_cache.dtype))
     if rc:
         _lib.check(rc, "afa_paged_commit")
+    increment_version((k_cache, v_cache))
     return lens

@@ -823,3 +823,34 @@ def test_strides_of_single_entries_do_not_matter(dtype):
     assert int(afa.paged_commit(*views, i32([[0]]), i32([2]), i32([8]), i32([[1, 3, -1]]))) == 4
     for t, b in zip(caches, before):
         assert torch.equal(t[0, 0, 2:4], b[0, 0, [3, 5]]) and torch.equal(t[0, 0, 4:], b[0, 0, 4:])
+
+
+def test_tensors_written_in_place_say_so():
+    """A backward pass that saved a tensor which one of the operators then changed is an error, not a wrong gradient."""
+    rng = np.random.default_rng(18)
+    caches = [dev(rng.standard_normal((4, 1, 16, 64)), F32) for _ in range(2)]
+    k = dev(rng.standard_normal((3, 1, 64)), F32)
+    table, free, one = i32([[0, 1, -1]]), i32([2, 3, 0]), i32([1])
+    out = torch.zeros((1, 1, 64), device="cuda")
+    path = i32([[1, 2]])
+    calls = {
+        "paged_append": (caches, lambda: afa.paged_append(k, k, *caches, dev([5, 6, 7]))),
+        "paged_commit": (caches, lambda: afa.paged_commit(*caches, table, one, i32([8]), path)),
+        "afa_paged": ([out], lambda: afa.afa_paged(k[:1], *caches, table, i32([8]), i32([0, 1]), out=out)),
+        "paged_plan": ([table, free], lambda: afa.paged_plan(table, i32([2]), i32([8]), i32([40]), free, i32([2]), 16,
+                                                             40)),
+    }
+    weight = torch.ones(8, device="cuda", requires_grad=True)
+    for name, (written, call) in calls.items():
+        for t in written:
+            y = (weight[0] * t).sum()
+            version = t._version
+            with torch.no_grad():
+                call()
+            assert t._version > version, name
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                y.backward()
+    with torch.inference_mode():
+        inside = [torch.zeros((4, 1, 16, 64), device="cuda") for _ in range(2)]
+        afa.paged_append(k, k, *inside, dev([5, 6, 7]))
+    afa.paged_append(k, k, *inside, dev([5, 6, 7]))
