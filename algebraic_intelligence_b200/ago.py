@@ -293,16 +293,17 @@ def apply_ago_rotations_axes(q, k, rotary_params, positions, sections):
     the same with its own number of heads. ``sections`` gives each axis (at most
     four) its channel pairs, in order: pair p of axis a at a token with
     ``positions[a, ..., token]`` = m turns by row m of the tables, pairs behind
-    the last section stay as they are. ``positions``: (axes, batch, tokens),
-    (axes, tokens) for packed inputs or the same positions in every batch row,
-    int32 or int64; one the tables do not hold is an error on the host and gives
-    NaN on the device. ``rotary_params`` as in ``apply_ago_rotations``, (positions,
-    dim / 2). Unlike there the tables keep their dtype: the arithmetic is
-    float32 (float64 for float64 inputs) with one rounding, which a bfloat16
-    table would limit to 2^-9. Differentiable in q and k by backward passes (before one
-    is captured into a CUDA graph, release what was computed from the same
-    leaves outside of it: PyTorch would wait for those leaves' stream). Returns
-    contiguous (q_rot, k_rot).
+    the last section stay as they are. Rows of q and k start on a channel pair
+    (views off one are refused; gradients off one are copied). ``positions``:
+    (axes, batch, tokens), (axes, tokens) for packed inputs or the same positions
+    in every batch row, int32 or int64; one the tables do not hold is an error on
+    the host and gives NaN on the device. ``rotary_params`` as in
+    ``apply_ago_rotations``, (positions, dim / 2). Unlike there the tables keep
+    their dtype: the arithmetic is float32 (float64 for float64 inputs) with one
+    rounding, which a bfloat16 table would limit to 2^-9. Differentiable in q and
+    k by backward passes (before one is captured into a CUDA graph, release what
+    was computed from the same leaves outside of it: PyTorch would wait for those
+    leaves' stream). Returns contiguous (q_rot, k_rot).
     """
     if q.ndim not in (3, 4):
         raise ValueError(f"q must have shape (batch, heads, tokens, dim) or (tokens, heads, dim), got {tuple(q.shape)}")

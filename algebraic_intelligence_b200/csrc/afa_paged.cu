@@ -33,9 +33,12 @@ namespace {
 constexpr int kSimtThreads = 256;
 
 // rho(s)^8 with rho(|s|) = |s| + sqrt(1 + s^2) and rho(-s) = 1 / rho(s): sums of
-// like signs only, correctly rounded root and quotient, so rho is within 1.5
-// half steps for every s and float32 weights within 16 (octic_ref's reciprocal
-// root alone is off by up to 2 steps).
+// like signs only, every operation correctly rounded. In half steps of the type
+// (relative): 1/2 of the fma's through the root, 1 the root's, 1 the sum's, and
+// for s < 0 1 the reciprocal's, so rho is within 2.5 or 3.5 and a weight, with
+// three squarings, within 8 times that plus 7: 27 or 35, 1.6e-6 or 2.1e-6 in
+// float32 (25 seen over 4M scores; octic_ref's reciprocal root alone is off by
+// up to 4).
 __device__ __forceinline__ float recip(float x) { return __frcp_rn(x); }
 __device__ __forceinline__ double recip(double x) { return __drcp_rn(x); }
 template <typename A>
@@ -61,9 +64,12 @@ struct alignas(16) Quad {
 // shared memory fall on different banks or are one broadcast, and there are few
 // of them for each FMA (6 to 32, 8 to 64 with 32 rows): the FMAs bound 32 rows,
 // the cache's bytes 8. Shared rows are DMAX channels padded by 16 bytes; several
-// CTAs per SM cover the loads' latency. Sums run over BN keys in registers of
-// their own before they join the row's, which keeps float32 results near 1e-7 at
-// any length.
+// CTAs per SM cover the loads' latency. Outputs add up over BN keys in registers
+// of their own before they join the row's, a thread's row sum takes TC weights a
+// step: few enough additions that they do not show. Float32 outputs and d_total
+// were 0.2e-6 to 2.6e-6 off (relative to sum p |v| and to d_total) from 64 to
+// 300000 keys, also 32768 of them in one CTA, without a trend in the length; a
+// score's rounding counts eightfold in its weight.
 template <typename A, int ROWS, int BN, int DMAX>
 struct SimtCfg {
   static constexpr int V = Quad<A>::N;

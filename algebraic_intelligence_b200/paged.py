@@ -218,9 +218,10 @@ def paged_append(k, v, k_cache, v_cache, slots, q=None, rotary_params=None, posi
     skipped, and slots inside it are distinct. With ``rotary_params``,
     ``positions`` (axes, tokens) and ``sections`` as in
     ``apply_ago_rotations_axes`` the keys are rotated, and so is ``q`` (tokens,
-    heads, dim), which comes back; without q the result is None. The caches may
-    be strided views (such as a (pages, page_size, heads, dim) cache
-    transposed) whose rows lie apart.
+    heads, dim), which comes back; without q the result is None. Rows start on a
+    channel pair (views off one are refused). The caches may be strided views
+    (such as a (pages, page_size, heads, dim) cache transposed) whose rows lie
+    apart.
     """
     pages, heads, page_size, dim = _caches(k_cache, v_cache)
     if k.ndim != 3 or k.shape != v.shape or k.shape[1:] != (heads, dim):
