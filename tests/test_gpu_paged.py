@@ -854,3 +854,104 @@ def test_tensors_written_in_place_say_so():
         inside = [torch.zeros((4, 1, 16, 64), device="cuda") for _ in range(2)]
         afa.paged_append(k, k, *inside, dev([5, 6, 7]))
     afa.paged_append(k, k, *inside, dev([5, 6, 7]))
+
+
+def exact(b, sink=0.5):
+    """(out, d_total, sum p |v| / d_total) of a Batch in float64, request by request, on the GPU."""
+    q, k, v, table, lens, cu, words = b.args()
+    group, page, dim = q.shape[1] // k.shape[1], k.shape[2], q.shape[2]
+    outs, dens, mags = [], [], []
+    for i, (n, length) in enumerate(zip(b.new.tolist(), b.lens.tolist())):
+        at = slice(int(b.cu[i]), int(b.cu[i]) + n)
+        pages = table[i, :-(-length // page)].long()
+        kk, vv = (x[pages].transpose(1, 2).reshape(-1, *x.shape[1::2])[:length].double().repeat_interleave(group, 1)
+                  for x in (k, v))
+        x = torch.einsum("nhd,lhd->nhl", q[at].double(), kk) / np.sqrt(dim)
+        node = torch.arange(length, device="cuda") - (length - n)
+        if words is None:
+            seen = node[None] <= torch.arange(n, device="cuda")[:, None]
+        else:
+            w = torch.nn.functional.pad(words[at].long(), (0, 9))[:, (node >> 5).clamp(min=0)]
+            seen = (node < 0)[None] | ((w >> (node & 31)) & 1).bool()
+        p = torch.exp(8 * torch.asinh(x)) * seen[:, None]
+        den = p.sum(-1) + sink
+        dens.append(den)
+        outs.append(torch.einsum("nhl,lhd->nhd", p, vv) / den[..., None])
+        mags.append(torch.einsum("nhl,lhd->nhd", p, vv.abs()) / den[..., None])
+    return torch.cat(outs), torch.cat(dens), torch.cat(mags)
+
+
+def check_exactly(b, weight, sink=0.5, **kw):
+    """Outputs within half a step of their type, and `weight` of sum p |v| for what the weights are off."""
+    got, gden = afa.afa_paged(*b.args(), sink_omega=sink, return_denominator=True, **kw)
+    assert _lib.device_status(got.device) == 0
+    want, den, mag = exact(b, sink)
+    t = want.shape[0]
+    half = torch.maximum(want.abs(), got[:t].double().abs()).log2().floor().exp2() * torch.finfo(got.dtype).eps / 2
+    off = ((got[:t].double() - want).abs() - half) / mag
+    assert off.max().item() <= weight
+    assert ((gden[:t].double() - den).abs() / den).max().item() <= min(weight, 3e-4)
+
+
+# What a weight is off in the tensor-core kernels, without its own rounding. The score: products of bfloat16 are
+# exact, their sum of at most 128 is off by sqrt(128) 2^-23 sum |q k| (under 110 for unit-normal numbers) / sqrt(128), and
+# rho^8 takes eight times that: 1.1e-4. The map: 2.5e-6 s^2, under 6e-5 for these scores. Two bfloat16 parts: 2^-17.
+# Together under 1.8e-4, bound 3e-4; a single bfloat16 weight adds half a step, 2^-8.
+SPLIT, SINGLE = 3e-4, 3e-4 + 2.0 ** -8
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("group", [1, 4, 7, 16])
+def test_attention_rows_of_few_keys(dim, group):
+    """Where roundings of single weights do not average out: requests of one to four keys, and trees on them. The
+    transposed kernel holds weights in two parts; the row-tile kernel, for 40 tokens a request, in one."""
+    lens = [1, 2, 3, 4] * 12
+    check_exactly(Batch(19, [1] * 48, lens, 2, group, dim, 16, BF), SPLIT)
+    two = 2 if group <= 16 else 1
+    check_exactly(Batch(20, [two] * 48, [x + two for x in lens], 2, group, dim, 16, BF, tree=True), SPLIT)
+    check_exactly(Batch(21, [40] * 6, [40, 41, 42, 43, 44, 40], 2, group, dim, 16, BF, tree=True), SINGLE)
+    check_exactly(Batch(22, [40] * 6, [40, 41, 42, 43, 44, 40], 2, group, dim, 16, BF), SINGLE)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("group", [1, 4, 7])
+@pytest.mark.parametrize("tree", [False, True])
+def test_attention_mixed_batch_in_64_bits(dim, group, tree):
+    """Single tokens, trees and chunks in one batch, and short and long requests of few rows, each row by itself."""
+    rng = np.random.default_rng(23)
+    new = rng.choice([1, 2, 7, 31, 33, 64, 65, 120, 200], 40)
+    check_exactly(Batch(24, new, new + rng.integers(0, 900, 40), 2, group, dim, 32, BF, tree=tree), SINGLE)
+    few = rng.choice([1, 1, 1, 2, 3], 60)
+    lens = np.where(rng.random(60) < 0.2, rng.integers(3, 5000, 60), rng.integers(3, 300, 60))
+    check_exactly(Batch(25, few, lens, 2, group, dim, 64, BF, tree=tree), SPLIT)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new,group", [(1, 4), (8, 4)])
+def test_attention_pieces_of_every_length_in_64_bits(dim, new, group):
+    lens = [max(new, 128 * (i % 9) + 1 + 37 * i % 128) for i in range(60)]
+    check_exactly(Batch(26, [new] * 60, lens, 3, group, dim, 128, BF), SPLIT)
+
+
+@pytest.mark.parametrize("dtype,weight", [(F32, 1e-5), (F64, 1e-13)])
+def test_attention_mixed_batch_on_cuda_cores_in_64_bits(dtype, weight):
+    """float32: the bound at the head of this file (a score is off by about 7e-7, its weight by eight times that: 5e-6,
+    bound 1e-5), here of each row's sum p |v| and not of the largest output. float64 2^-29 of that on either side:
+    4e-14, bound 1e-13."""
+    rng = np.random.default_rng(27)
+    new = rng.choice([1, 2, 7, 31, 33, 64], 20)
+    for dim in (64, 100, 128):
+        check_exactly(Batch(28, new, new + rng.integers(0, 600, 20), 2, 5, dim, 32, dtype, tree=True), weight)
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF, 128), (BF, 64), (F32, 64)])
+@pytest.mark.parametrize("name", ["decode", "odd-group", "chunk", "tree", "wide-tree", "long-tree"])
+def test_attention_into_its_queries(name, dtype, dim):
+    """A unit's rows are read before they are written, and by no other unit."""
+    b = Batch(29, dim=dim, dtype=dtype, **CASES[name])
+    want = afa.afa_paged(*b.args())
+    for _ in range(3):
+        q, *rest = b.args()
+        q = q.clone()
+        assert afa.afa_paged(q, *rest, out=q) is q
+        assert torch.equal(q, want)
