@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import numpy as np
 import torch
-from torch.autograd.forward_ad import unpack_dual
+from torch.autograd import forward_ad
 
 
 class Staged:
@@ -58,8 +58,13 @@ def host_checks_float(*arrays) -> None:
             raise TypeError("expected a floating point array")
 
 
+def tangents_exist() -> bool:
+    """Whether a forward-mode level is open: asking each tensor for a tangent takes 0.3 us."""
+    return forward_ad._current_level >= 0
+
+
 def refuse_tangents(what, *arrays) -> None:
     """ValueError for inputs with a forward-mode tangent, which a kernel would drop without a sign."""
     for a in arrays:
-        if isinstance(a, torch.Tensor) and unpack_dual(a).tangent is not None:
+        if isinstance(a, torch.Tensor) and forward_ad.unpack_dual(a).tangent is not None:
             raise ValueError(f"{what} has no forward-mode derivative")

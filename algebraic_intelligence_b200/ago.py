@@ -29,7 +29,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._tensors import Staged, host_checks_float, refuse_tangents
+from ._tensors import Staged, host_checks_float, refuse_tangents, tangents_exist
 
 __all__ = ["CayleyRotary", "build_cayley_rotary_matrix", "apply_ago_rotations", "apply_ago_rotations_axes"]
 
@@ -206,7 +206,8 @@ def axis_arguments(rotary_params, positions, sections, dim, shape, device) -> Ax
                          f"{tuple(s.shape)}")
     if c.requires_grad or s.requires_grad:
         raise ValueError("the rotary tables have no gradient")
-    refuse_tangents("a rotary table", c, s)
+    if tangents_exist():
+        refuse_tangents("a rotary table", c, s)
     p = positions if isinstance(positions, torch.Tensor) else torch.as_tensor(np.asarray(positions))
     if p.dtype != torch.int32 and p.dtype != torch.int64:
         raise TypeError("positions must be int32 or int64")
@@ -317,7 +318,8 @@ def apply_ago_rotations_axes(q, k, rotary_params, positions, sections):
     if q.shape[head] == 0 or (k is not None and k.shape[head] == 0):
         raise ValueError("q and k need at least one head")
     host_checks_float(*(t for t in (q, k) if t is not None))
-    refuse_tangents("apply_ago_rotations_axes", q, k)
+    if tangents_exist():
+        refuse_tangents("apply_ago_rotations_axes", q, k)
     if k is not None and k.dtype != q.dtype:
         raise TypeError("q and k must share a dtype")
     on_gpu = all(t is None or (isinstance(t, torch.Tensor) and t.is_cuda) for t in (q, k))

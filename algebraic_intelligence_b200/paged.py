@@ -31,7 +31,7 @@ import torch
 from torch.autograd.graph import increment_version
 
 from . import _lib
-from ._tensors import refuse_tangents
+from ._tensors import refuse_tangents, tangents_exist
 from .ago import axis_arguments
 
 __all__ = ["PagedPlan", "paged_plan", "paged_append", "afa_paged", "paged_commit", "paged_workspace_bytes"]
@@ -81,7 +81,8 @@ def _no_gradient(what, *tensors):
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise ValueError(f"{what} has no gradient: call it under torch.no_grad()")
-    refuse_tangents(what, *tensors)
+    if tangents_exist():
+        refuse_tangents(what, *tensors)
 
 
 def _caches(k_cache, v_cache, ndims=(4,)):
@@ -120,9 +121,11 @@ def _apart(shape, strides, behind) -> bool:
 
 def _written(k_cache, v_cache):
     """Refuses caches whose rows share memory, as an expanded one's: moves and writes of rows would race."""
-    behind = abs(k_cache.data_ptr() - v_cache.data_ptr()) // k_cache.element_size()
+    behind = abs(k_cache.data_ptr() - v_cache.data_ptr())
+    if k_cache.is_contiguous() and v_cache.is_contiguous() and behind >= k_cache.nbytes:
+        return
     if k_cache.stride() == v_cache.stride():
-        apart = _apart(k_cache.shape, k_cache.stride(), behind)
+        apart = _apart(k_cache.shape, k_cache.stride(), behind // k_cache.element_size())
     else:
         apart = behind > 0 and all(_apart(t.shape, t.stride(), 1 << 62) for t in (k_cache, v_cache))
     if not apart:
