@@ -336,11 +336,15 @@ def apply_ago_rotations_axes(q, k, rotary_params, positions, sections):
     if qt.dtype not in _TABLE_DTYPES:
         raise TypeError("q and k must be float32, bfloat16 or float64")
     axes = axis_arguments(rotary_params, positions, sections, dim, _axis_shape(qt, positions), qt.device)
-    if torch.is_grad_enabled() and (qt.requires_grad or (kt is not None and kt.requires_grad)):
-        outs = _RotateAxes.apply(qt, kt, *axes, False)
-        outs = (outs, None) if kt is None else outs
-    else:
+    if not torch.is_grad_enabled() or not (qt.requires_grad or (kt is not None and kt.requires_grad)):
         outs = _rotate_axes(qt, kt, axes, False)
+    elif kt is None:
+        outs = _RotateAxes.apply(qt, None, *axes, False), None
+    elif qt.requires_grad and kt.requires_grad:
+        outs = _RotateAxes.apply(qt, kt, *axes, False)
+    else:  # together both results would want a gradient
+        outs = tuple(_RotateAxes.apply(t, None, *axes, False) if t.requires_grad else
+                     _rotate_axes(t, None, axes, False)[0] for t in (qt, kt))
     return tuple(outs) if st is None else (st.back(outs[0]), st.back(outs[1]))
 
 

@@ -955,3 +955,18 @@ def test_attention_into_its_queries(name, dtype, dim):
         q = q.clone()
         assert afa.afa_paged(q, *rest, out=q) is q
         assert torch.equal(q, want)
+
+
+def test_rotation_of_one_input_that_wants_a_gradient():
+    """The other's result wants none, and both have the bits of a rotation together."""
+    rng = np.random.default_rng(30)
+    c, s = tables(32, 16, F32)
+    pos, up = dev(rng.integers(0, 16, (2, 1, 7))), dev(rng.standard_normal((1, 4, 7, 32)), F32)
+    x, y = (dev(rng.standard_normal((1, h, 7, 32)), F32) for h in (4, 2))
+    want = afa.apply_ago_rotations_axes(x, y, (c, s), pos, (7, 9))
+    back, = torch.autograd.grad(afa.apply_ago_rotations_axes(x.requires_grad_(True), None, (c, s), pos, (7, 9))[0], x, up)
+    qr, kr = afa.apply_ago_rotations_axes(x, y, (c, s), pos, (7, 9))
+    assert qr.requires_grad and not kr.requires_grad and torch.equal(qr, want[0]) and torch.equal(kr, want[1])
+    assert torch.equal(torch.autograd.grad(qr, x, up)[0], back)
+    kr, qr = afa.apply_ago_rotations_axes(y, x, (c, s), pos, (7, 9))
+    assert qr.requires_grad and not kr.requires_grad and torch.equal(torch.autograd.grad(qr, x, up)[0], back)
