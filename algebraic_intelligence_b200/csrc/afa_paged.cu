@@ -68,8 +68,9 @@ struct alignas(16) Quad {
 // of their own before they join the row's, a thread's row sum takes TC weights a
 // step: few enough additions that they do not show. Float32 outputs and d_total
 // were 0.2e-6 to 2.6e-6 off (relative to sum p |v| and to d_total) from 64 to
-// 300000 keys, also 32768 of them in one CTA, without a trend in the length; a
-// score's rounding counts eightfold in its weight.
+// 300000 keys of 64 and 128 channels, also 32768 of them in one CTA, without a
+// trend in the length (up to 1.3e-5 with 256 channels: a score's rounding counts
+// eightfold in its weight).
 template <typename A, int ROWS, int BN, int DMAX>
 struct SimtCfg {
   static constexpr int V = Quad<A>::N;
