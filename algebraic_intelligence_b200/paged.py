@@ -110,13 +110,20 @@ def _caches(k_cache, v_cache, ndims=(4,)):
 def _apart(shape, strides, behind) -> bool:
     """Whether the elements of a strided view, and of a second one ``behind`` elements further, all lie apart. (Views
     made by slicing, indexing and transposing do: each stride passes what the smaller ones span.)"""
-    span = 0
-    for stride, n in sorted((*zip(strides, shape), (behind, 2))):
-        if n > 1:
-            if stride <= span:
-                return False
-            span += stride * (n - 1)
-    return True
+    def nested(*axes):
+        span = 0
+        for stride, n in sorted(axes):
+            if n > 1:
+                if stride <= span:
+                    return False
+                span += stride * (n - 1)
+        return True
+
+    axes = tuple(zip(strides, shape))
+    # Or the second lies between the first's rows of an axis, some rows on (odd pages behind even ones).
+    return nested(*axes, (behind, 2)) or any(
+        nested(*axes[:i], (stride, n + behind // stride), *axes[i + 1:], (behind % stride, 2))
+        for i, (stride, n) in enumerate(axes) if n > 1 and 0 < stride < behind)
 
 
 def _written(k_cache, v_cache):

@@ -312,12 +312,13 @@ def test_caches_whose_rows_share_memory_are_refused(layers, monkeypatch):
     calls = [_commit] if layers else [_commit, _append]
     plain = z(5, 2, 16, 8)
     wide = z(5, 2, 2, 16, 8)
-    fused, pool = z(5, 16, 2, 24), z(10, 2, 16, 8)
+    fused, pool, far = z(5, 16, 2, 24), z(10, 2, 16, 8), z(18, 2, 16, 8)
     for k, v in ((plain, z(5, 2, 16, 8)), (z(5, 16, 2, 8).transpose(-3, -2), z(5, 16, 2, 8).transpose(-3, -2)),
                  (z(5, 16, 2, 8).transpose(-3, -2), plain), (wide.select(-4, 0), wide.select(-4, 1)),
                  (wide.select(-4, 1), wide.select(-4, 0)), (wide.select(-3, 0), wide.select(-3, 1)),
                  (fused[..., :8].transpose(-3, -2), fused[..., 16:].transpose(-3, -2)),
-                 (pool[..., ::2, :, :, :], pool[..., 1::2, :, :, :]), (pool[..., 5:, :, :, :], pool[..., :5, :, :, :])):
+                 (pool[..., ::2, :, :, :], pool[..., 1::2, :, :, :]), (pool[..., 5:, :, :, :], pool[..., :5, :, :, :]),
+                 (far[..., :10:2, :, :, :], far[..., 5:15:2, :, :, :]), (far[..., 9::2, :, :, :], far[..., :10:2, :, :, :])):
         for call in calls:
             with pytest.raises(Launched):
                 call(k_cache=k, v_cache=v)
@@ -325,7 +326,8 @@ def test_caches_whose_rows_share_memory_are_refused(layers, monkeypatch):
     pages = z(1, 2, 16, 8).expand(*lead, 5, 2, 16, 8)
     window = torch.zeros(4000).as_strided((*lead, 5, 2, 16, 8), (*(2000,) * len(lead), 256, 128, 4, 1))
     for k, v in ((spread, plain), (plain, pages), (plain, plain), (plain, window), (window, window),
-                 (wide.select(-4, 0), wide.select(-4, 0)), (spread, spread)):
+                 (wide.select(-4, 0), wide.select(-4, 0)), (spread, spread), (pool[..., :5, :, :, :], pool[..., 4:9, :, :, :]),
+                 (far[..., :10:2, :, :, :], far[..., 4:14:2, :, :, :])):
         for call in calls:
             with pytest.raises(ValueError, match="share memory"):
                 call(k_cache=k, v_cache=v)
